@@ -13,7 +13,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
-SOURCES = ["disco_spmm.hip", "disco_stream.hip", "disco_schedule.hip", "disco_norm.hip", "disco_scorer.hip", "disco_build.hip", "disco_gather.hip", "disco_locality.hip"]
+SOURCES = ["disco_spmm.hip", "disco_stream.hip", "disco_schedule.hip", "disco_norm.hip", "disco_scorer.hip",
+           "disco_build.hip", "disco_gather.hip", "disco_locality.hip"]
 HEADERS = ["disco_internal.h", "disco_spmm_common.h", os.path.join(ROOT, "include", "disco_hip.h")]
 ARCH = "gfx950"
 
@@ -42,14 +43,22 @@ def build_lib(force: bool = False, extra_flags=(), name: str = "libdisco_hip.so"
         return out
     hipcc = _hipcc()
     flags = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-fhip-fp32-correctly-rounded-divide-sqrt",
-             "-ffp-contract=off", "-Wall", "-Wno-unused-function", f"-I{os.path.join(ROOT, 'include')}", f"-I{CSRC}"]
+             "-ffp-contract=off", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+             "-Wall", "-Wno-unused-function", f"-I{os.path.join(ROOT, 'include')}", f"-I{CSRC}"]
+    # -packed-fp32-ops (the host pass warns that it does not know the feature): some forms of the packed float32
+    # instructions that hipcc makes from ordinary float code have given wrong results on MI355X now and then
     flags += list(extra_flags)
     objdir = os.path.join(CSRC, "build", name.replace(".so", ""))
     os.makedirs(objdir, exist_ok=True)
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
 
+    def needs(src: str):
+        return [os.path.abspath(__file__), os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS]
+
     def compile_one(src: str) -> str:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))
+        if not force and not extra_flags and os.path.exists(obj) and os.path.getmtime(obj) >= max(map(os.path.getmtime, needs(src))):
+            return obj
         cmd = [hipcc, *flags, "-c", os.path.join(CSRC, src), "-o", obj]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
