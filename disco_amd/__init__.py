@@ -5,6 +5,7 @@ Host side mirrors the reference's Python module API (``models.convs_large``, ``u
 behind the C ABI of ``include/disco_hip.h`` (``disco_amd/csrc/libdisco_hip.so``).
 """
 from .sparse import SparseTensor  # noqa: F401
-from .ops import khop, matmul, max_aggregate, pair_gather, spmm  # noqa: F401
+from .ops import (clip_grad_norm_, clip_grads, grad_norm, khop, matmul, max_aggregate, pair_gather, residual_norm,  # noqa: F401
+                  row_norm, spmm)
 
 __version__ = "0.1.0"

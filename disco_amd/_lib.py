@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 
-import torch  # noqa: F401  (loads the process's HIP runtime before our library binds to it)
+import torch  # (loads the process's HIP runtime before our library binds to it)
 
 from .build import lib_path
 
@@ -25,6 +25,22 @@ class ScheduleInfo(C.Structure):
         "n_multi_rows", "max_row_nnz", "off_perm", "off_piece_row", "off_piece_begin", "off_piece_end",
         "off_piece_slot", "off_multi_row", "off_multi_first", "ws_bytes",
         "sweep_windows", "sweep_window_rows", "sweep_count_padded", "sweep_n_cols")] + [("sweep_ws", C.c_void_p), ("n_cols", C.c_int64), ("xcd_run", C.c_int64)]
+
+
+class ResidualNorm(C.Structure):
+    """Mirror of ``disco_residual_norm`` (include/disco_hip.h)."""
+    _fields_ = ([(n, C.c_int64) for n in ("rows", "width", "ldx", "ldy", "ld_gate")]
+                + [(n, C.c_void_p) for n in ("x", "y", "gate", "post_weight", "post_bias", "pre_weight", "pre_bias", "scale_vector")]
+                + [(n, C.c_int32) for n in ("stream_type", "block_type", "param_type", "has_block", "post_norm", "pre_norm",
+                                            "gate_kind", "gate_act")]
+                + [("scale", C.c_float), ("eps", C.c_float)])
+
+
+class ResidualNormGrads(C.Structure):
+    """Mirror of ``disco_residual_norm_grads`` (include/disco_hip.h)."""
+    _fields_ = ([(n, C.c_void_p) for n in ("dout", "dh", "dx", "dy", "dgate")]
+                + [(n, C.c_int64) for n in ("ld_dout", "ld_dh", "ld_dx", "ld_dy", "ld_dgate")]
+                + [(n, C.c_void_p) for n in ("dpost_weight", "dpost_bias", "dpre_weight", "dpre_bias", "dscale")])
 
 
 _SIGNATURES = {
@@ -80,7 +96,17 @@ _SIGNATURES = {
                                      c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "disco_pair_gather_f32": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                                       c_void_p, c_int64, c_void_p, c_void_p]),
+    "disco_residual_norm_forward": (c_int, [C.POINTER(ResidualNorm), c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "disco_residual_norm_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "disco_residual_norm_backward": (c_int, [C.POINTER(ResidualNorm), c_void_p, C.POINTER(ResidualNormGrads), c_void_p, c_size_t,
+                                             c_void_p]),
+    "disco_grad_norm_workspace_bytes": (c_size_t, [c_int64]),
+    "disco_grad_norm": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "disco_grad_clip": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, C.c_double, c_void_p, c_void_p,
+                                c_size_t, c_void_p]),
 }
+RESIDUAL_MAX_WIDTH = 16384
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # disco_dtype
 NOALLOC_SCRATCH_BYTES = 16 << 20
 COO_SYMMETRISE, COO_DUP_KEEP, COO_DUP_SUM, COO_DUP_FIRST = 1, 0, 2, 4
 

@@ -14,8 +14,10 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 ROOT = os.path.dirname(HERE)
 SOURCES = ["disco_spmm.hip", "disco_stream.hip", "disco_schedule.hip", "disco_norm.hip", "disco_scorer.hip",
-           "disco_build.hip", "disco_gather.hip", "disco_locality.hip"]
-HEADERS = ["disco_internal.h", "disco_spmm_common.h", os.path.join(ROOT, "include", "disco_hip.h")]
+           "disco_build.hip", "disco_gather.hip", "disco_locality.hip",
+           "disco_gradnorm.hip", "disco_residual.hip", "disco_residual_f32.hip", "disco_residual_f16.hip", "disco_residual_bf16.hip",
+           "disco_residual_f32_f16.hip", "disco_residual_f32_bf16.hip"]
+HEADERS = ["disco_internal.h", "disco_spmm_common.h", "disco_residual.h", os.path.join(ROOT, "include", "disco_hip.h")]
 ARCH = "gfx950"
 
 
@@ -53,7 +55,8 @@ def build_lib(force: bool = False, extra_flags=(), name: str = "libdisco_hip.so"
     srcs = [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
 
     def needs(src: str):
-        return [os.path.abspath(__file__), os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in HEADERS]
+        heads = [h for h in HEADERS if h != "disco_residual.h" or src.startswith("disco_residual")]
+        return [os.path.abspath(__file__), os.path.join(CSRC, src)] + [os.path.join(CSRC, h) for h in heads]
 
     def compile_one(src: str) -> str:
         obj = os.path.join(objdir, src.replace(".hip", ".o"))

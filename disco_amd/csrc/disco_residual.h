@@ -1,0 +1,396 @@
+// Kernels of the join between two residual blocks (forward and backward), one instantiation unit per pair of types.
+//
+//   z   = u1 * w1 + b1,  u1 = standardised row of y           (post norm: rms, layer or none -> z = y)
+//   out = x + lam * a * z,  lam = scale (* channel gate),  a = act(gate) per element or per row
+//   h   = u2 * w2 + b2,  u2 = standardised row of out         (pre norm of the next block: rms, layer or none)
+//
+// Backward, with q = dh * w2 and m(.) the mean over the row:
+//   dO = dout + r2 * (q - m(q) - u2 * m(q * u2))              (rms: without the m(q) term)
+//   dx = dO,  p = dO * a * lam * w1,  dy = r1 * (p - m(p) - u1 * m(p * u1)),  dgate = dO * lam * z * a'
+//   Every parameter gradient is a column sum, and four of them are enough:
+//   P1 = sum dO * a * u1,  P2 = sum dO * a,  P3 = sum dh * u2,  P4 = sum dh   (k_residual_finish derives the rest).
+//
+// Both directions are bound by memory (about 20 and 40 operations for 20 to 40 bytes): a row is read once into registers,
+// all its reductions run there, and each output is written once.  Statistics and sums are float32 whatever the types;
+// values are rounded once, when they are stored.  The next block's norm reads the unrounded sum, not the stored one: its
+// only rounding is then its own, and the backward, which rebuilds the sum from x and y, sees the same values.
+#ifndef DISCO_RESIDUAL_H
+#define DISCO_RESIDUAL_H
+
+#include "disco_internal.h"
+
+namespace disco {
+
+struct ResidualArgs {
+  int64_t rows, ldx, ldy, ldg, ldo, ldh;
+  int64_t lddo, lddh, lddx, lddy, lddg;
+  int width, param_type, post, pre, gate, act;
+  float scale, eps, inv_width;
+  const void *x, *y, *g, *w1, *b1, *w2, *b2, *lam;
+  void *out, *h;
+  float* stats;                     // [4, rows]: mean and 1 / deviation of y, then of the sum; NULL: not kept
+  const void *dout, *dh;
+  void *dx, *dy, *dg;
+  float* partial;                   // [workgroups, 4, width]: column sums of each workgroup; NULL: no parameter gradient
+  int partials;                     // bit k: sum P(k+1) is wanted
+};
+
+enum ResidualPair { kPairF32 = 0, kPairF16 = 1, kPairBF16 = 2, kPairF32F16 = 3, kPairF32BF16 = 4 };
+
+// A kernel variant: lanes per row and elements a lane holds; the workgroup has 256 lanes, or a row's if those are more.
+struct ResidualShape { int lanes, elems, threads; };
+inline ResidualShape residual_shape(int64_t width) {
+  const int table[][2] = {{16, 4}, {32, 4}, {64, 4}, {64, 8}, {64, 12}, {64, 16}, {256, 8}, {256, 16}, {512, 16}, {1024, 16}};
+  for (const auto& t : table)
+    if (width <= (int64_t)t[0] * t[1]) return {t[0], t[1], t[0] > 256 ? t[0] : 256};
+  return {0, 0, 0};
+}
+
+// grid: workgroups; a workgroup takes rows / (its rows at a time * grid) turns
+template <int PAIR> int residual_forward(const ResidualArgs& a, unsigned grid, hipStream_t stream);
+template <int PAIR> int residual_backward(const ResidualArgs& a, unsigned grid, hipStream_t stream);
+
+#if defined(DISCO_RESIDUAL_KERNELS)
+
+template <int T> struct TypeOf;
+template <> struct TypeOf<DISCO_F32> { typedef float type; };
+template <> struct TypeOf<DISCO_F16> { typedef _Float16 type; };
+template <> struct TypeOf<DISCO_BF16> { typedef __bf16 type; };
+
+__device__ __forceinline__ float load_param(const void* p, int type, int64_t i) {
+  if (type == DISCO_F32) return static_cast<const float*>(p)[i];
+  if (type == DISCO_F16) return (float)static_cast<const _Float16*>(p)[i];
+  return (float)static_cast<const __bf16*>(p)[i];
+}
+
+__device__ __forceinline__ float activate(float g, int act) {
+  if (act == DISCO_ACT_SIGMOID) return 1.0f / (1.0f + expf(-g));
+  if (act == DISCO_ACT_TANH) return tanhf(g);
+  return g;
+}
+// derivative from the activation's own value
+__device__ __forceinline__ float activate_slope(float a, int act) {
+  if (act == DISCO_ACT_SIGMOID) return a * (1.0f - a);
+  if (act == DISCO_ACT_TANH) return 1.0f - a * a;
+  return 1.0f;
+}
+
+// One lane's part of a row: vectors of four elements, `lanes` vectors apart.  Rows may start at any element: the vector
+// type asks for the element's alignment only, which global memory instructions allow.  ODD: the width is no multiple of
+// four, so the row's last vector is partial.
+template <typename T, int LANES, int E, bool ODD>
+struct RowPart {
+  typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+  __device__ static __forceinline__ void load(float (&r)[E], const T* p, int lane, int width) {
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k) {
+      const int c = (k * LANES + lane) * 4;
+      vec v = {};
+      if (c + 4 <= width) {
+        v = *reinterpret_cast<const vec*>(p + c);
+      } else if (ODD && c < width) {
+        v.x = p[c];
+        if (c + 1 < width) v.y = p[c + 1];
+        if (c + 2 < width) v.z = p[c + 2];
+      }
+      r[4 * k] = (float)v.x; r[4 * k + 1] = (float)v.y; r[4 * k + 2] = (float)v.z; r[4 * k + 3] = (float)v.w;
+    }
+  }
+  __device__ static __forceinline__ void store(const float (&r)[E], T* p, int lane, int width) {
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k) {
+      const int c = (k * LANES + lane) * 4;
+      vec v;
+      v.x = (T)r[4 * k]; v.y = (T)r[4 * k + 1]; v.z = (T)r[4 * k + 2]; v.w = (T)r[4 * k + 3];
+      if (c + 4 <= width) {
+        *reinterpret_cast<vec*>(p + c) = v;
+      } else if (ODD && c < width) {
+        p[c] = v.x;
+        if (c + 1 < width) p[c + 1] = v.y;
+        if (c + 2 < width) p[c + 2] = v.z;
+      }
+    }
+  }
+};
+
+// Sums R values over the lanes of a row, the same in every lane.  The order is fixed: results do not vary from run to run.
+template <int LANES, int R>
+__device__ __forceinline__ void row_sum(float (&v)[R], float* lds, int& turn) {
+  constexpr int IN_WAVE = LANES < 64 ? LANES : 64;
+#pragma unroll
+  for (int o = IN_WAVE / 2; o > 0; o >>= 1)
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] += __shfl_xor(v[r], o, 64);
+  if constexpr (LANES > 64) {
+    constexpr int WAVES = LANES / 64;
+    // two buffers in turn: a wave that is ahead by one reduction writes the other one, and cannot be ahead by two
+    float* part = lds + turn * (WAVES * 4);
+    turn ^= 1;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int r = 0; r < R; ++r) part[(threadIdx.x >> 6) * 4 + r] = v[r];
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float s = 0.0f;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) s += part[w * 4 + r];
+      v[r] = s;
+    }
+  }
+}
+
+template <int E, int LANES>
+__device__ __forceinline__ bool in_row(int e, int lane, int width) { return ((e >> 2) * LANES + lane) * 4 + (e & 3) < width; }
+
+// Standardises a row in place and returns (mean, 1 / deviation).  The variance is summed from the deviations, after the
+// mean: subtracting two large sums would lose it.  Elements behind the width stay zero.
+template <int LANES, int E>
+__device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, float inv_width, int lane, int width, float* lds,
+                                            int& turn, float& mean, float& rstd) {
+  float s[1] = {0.0f};
+  mean = 0.0f;
+  if (kind == DISCO_NORM_LAYER) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s[0] += v[e];
+    row_sum<LANES, 1>(s, lds, turn);
+    mean = s[0] * inv_width;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = in_row<E, LANES>(e, lane, width) ? v[e] - mean : 0.0f;
+    s[0] = 0.0f;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e) s[0] = fmaf(v[e], v[e], s[0]);
+  row_sum<LANES, 1>(s, lds, turn);
+  rstd = 1.0f / sqrtf(fmaf(s[0], inv_width, eps));
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] *= rstd;
+}
+
+// z = u1 * A + B with the residual scale and a channel gate folded in (A = lam * w1, B = lam * b1): loaded once per workgroup.
+template <int LANES, int E>
+__device__ __forceinline__ void load_branch(const ResidualArgs& a, int lane, float (&A)[E], float (&B)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int c = ((e >> 2) * LANES + lane) * 4 + (e & 3);
+    float lam = a.scale;
+    A[e] = B[e] = 0.0f;
+    if (c < a.width) {
+      if (a.lam) lam *= load_param(a.lam, a.param_type, c);
+      if (a.gate == DISCO_GATE_CHANNEL) lam *= activate(load_param(a.g, a.param_type, c), a.act);
+      A[e] = a.w1 ? lam * load_param(a.w1, a.param_type, c) : lam;
+      if (a.b1) B[e] = lam * load_param(a.b1, a.param_type, c);
+    }
+  }
+}
+
+template <int LANES, int E>
+__device__ __forceinline__ void load_vector(const void* p, int type, int lane, int width, float other, float (&v)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int c = ((e >> 2) * LANES + lane) * 4 + (e & 3);
+    v[e] = p && c < width ? load_param(p, type, c) : other;
+  }
+}
+
+template <typename TX, typename TY, int LANES, int E, bool ODD>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_forward(const ResidualArgs a) {
+  constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
+  __shared__ float lds[2 * (THREADS / 64) * 4];
+  const int lane = threadIdx.x % LANES;
+  int turn = 0;
+  float A[E], B[E], W2[E], B2[E];
+  if (a.y) load_branch<LANES, E>(a, lane, A, B);
+  if (a.pre) {
+    load_vector<LANES, E>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
+    load_vector<LANES, E>(a.b2, a.param_type, lane, a.width, 0.0f, B2);
+  }
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+    float o[E];
+    RowPart<TX, LANES, E, ODD>::load(o, static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
+    if (a.y) {
+      float z[E], g[E], grow = 1.0f, mean, rstd;
+      RowPart<TY, LANES, E, ODD>::load(z, static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
+      if (a.gate == DISCO_GATE_FULL) RowPart<TY, LANES, E, ODD>::load(g, static_cast<const TY*>(a.g) + row * a.ldg, lane, a.width);
+      if (a.gate == DISCO_GATE_ROW) grow = activate((float)static_cast<const TY*>(a.g)[row * a.ldg], a.act);
+      if (a.post) {
+        standardise<LANES, E>(z, a.post, a.eps, a.inv_width, lane, a.width, lds, turn, mean, rstd);
+        if (a.stats && lane == 0) { a.stats[row] = mean; a.stats[a.rows + row] = rstd; }
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float t = fmaf(z[e], A[e], B[e]);
+        if (a.gate == DISCO_GATE_FULL) t *= activate(g[e], a.act);
+        if (a.gate == DISCO_GATE_ROW) t *= grow;
+        o[e] += t;
+      }
+      RowPart<TX, LANES, E, ODD>::store(o, static_cast<TX*>(a.out) + row * a.ldo, lane, a.width);
+    }
+    if (a.pre) {
+      float mean, rstd;
+      standardise<LANES, E>(o, a.pre, a.eps, a.inv_width, lane, a.width, lds, turn, mean, rstd);
+      if (a.stats && lane == 0) { a.stats[2 * a.rows + row] = mean; a.stats[3 * a.rows + row] = rstd; }
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], W2[e], B2[e]);
+      RowPart<TY, LANES, E, ODD>::store(o, static_cast<TY*>(a.h) + row * a.ldh, lane, a.width);
+    }
+  }
+}
+
+template <typename TX, typename TY, int LANES, int E, bool ODD>
+__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward(const ResidualArgs a) {
+  constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
+  __shared__ float lds[2 * (THREADS / 64) * 4];
+  __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
+  const int lane = threadIdx.x % LANES;
+  int turn = 0;
+  float A[E], B[E], W2[E], P1[E], P2[E], P3[E], P4[E];
+  if (a.y) load_branch<LANES, E>(a, lane, A, B);
+  if (a.pre) load_vector<LANES, E>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
+#pragma unroll
+  for (int e = 0; e < E; ++e) P1[e] = P2[e] = P3[e] = P4[e] = 0.0f;
+  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+    float u1[E], act[E], d[E], r1 = 1.0f, grow = 1.0f;
+    if (a.y) {
+      RowPart<TY, LANES, E, ODD>::load(u1, static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
+      if (a.gate == DISCO_GATE_FULL) RowPart<TY, LANES, E, ODD>::load(act, static_cast<const TY*>(a.g) + row * a.ldg, lane, a.width);
+      if (a.gate == DISCO_GATE_ROW) grow = activate((float)static_cast<const TY*>(a.g)[row * a.ldg], a.act);
+      if (a.post) {
+        const float mean = a.stats[row];
+        r1 = a.stats[a.rows + row];
+#pragma unroll
+        for (int e = 0; e < E; ++e) u1[e] = in_row<E, LANES>(e, lane, a.width) ? (u1[e] - mean) * r1 : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) act[e] = a.gate == DISCO_GATE_FULL ? activate(act[e], a.act) : grow;
+    }
+    if (a.dout) {
+      RowPart<TX, LANES, E, ODD>::load(d, static_cast<const TX*>(a.dout) + row * a.lddo, lane, a.width);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) d[e] = 0.0f;
+    }
+    if (a.dh) {
+      float u2[E], q[E], s[2] = {0.0f, 0.0f};
+      RowPart<TX, LANES, E, ODD>::load(u2, static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
+      RowPart<TY, LANES, E, ODD>::load(q, static_cast<const TY*>(a.dh) + row * a.lddh, lane, a.width);
+      const float mean = a.stats[2 * a.rows + row], r2 = a.stats[3 * a.rows + row];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (a.y) u2[e] = fmaf(act[e], fmaf(u1[e], A[e], B[e]), u2[e]);
+        u2[e] = in_row<E, LANES>(e, lane, a.width) ? (u2[e] - mean) * r2 : 0.0f;
+        P3[e] = fmaf(q[e], u2[e], P3[e]);
+        P4[e] += q[e];
+        q[e] *= W2[e];
+        s[0] = fmaf(q[e], u2[e], s[0]);
+        s[1] += q[e];
+      }
+      row_sum<LANES, 2>(s, lds, turn);
+      const float mq = a.pre == DISCO_NORM_LAYER ? s[1] * a.inv_width : 0.0f, mqu = s[0] * a.inv_width;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        d[e] += in_row<E, LANES>(e, lane, a.width) ? r2 * (q[e] - mq - u2[e] * mqu) : 0.0f;
+    }
+    if (a.dx) RowPart<TX, LANES, E, ODD>::store(d, static_cast<TX*>(a.dx) + row * a.lddx, lane, a.width);
+    if (a.y) {
+      float s[3] = {0.0f, 0.0f, 0.0f};
+      float dg[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float t = d[e] * fmaf(u1[e], A[e], B[e]);
+        s[2] += t;
+        dg[e] = t * activate_slope(act[e], a.act);
+        d[e] *= act[e];
+        P1[e] = fmaf(d[e], u1[e], P1[e]);
+        P2[e] += d[e];
+        d[e] *= A[e];
+        s[0] = fmaf(d[e], u1[e], s[0]);
+        s[1] += d[e];
+      }
+      if (a.dg && a.gate == DISCO_GATE_FULL)
+        RowPart<TY, LANES, E, ODD>::store(dg, static_cast<TY*>(a.dg) + row * a.lddg, lane, a.width);
+      if (a.post || (a.dg && a.gate == DISCO_GATE_ROW)) row_sum<LANES, 3>(s, lds, turn);
+      if (a.dg && a.gate == DISCO_GATE_ROW && lane == 0)
+        static_cast<TY*>(a.dg)[row * a.lddg] = (TY)(s[2] * activate_slope(grow, a.act));
+      if (a.dy) {
+        if (a.post) {
+          const float mp = a.post == DISCO_NORM_LAYER ? s[1] * a.inv_width : 0.0f, mpu = s[0] * a.inv_width;
+#pragma unroll
+          for (int e = 0; e < E; ++e) d[e] = r1 * (d[e] - mp - u1[e] * mpu);
+        }
+        RowPart<TY, LANES, E, ODD>::store(d, static_cast<TY*>(a.dy) + row * a.lddy, lane, a.width);
+      }
+    }
+  }
+  if (!a.partial) return;
+  // column sums of the workgroup: its ROWS row groups in order, then one partial row per sum
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if (!(a.partials >> k & 1)) continue;
+    const float* P = k == 0 ? P1 : k == 1 ? P2 : k == 2 ? P3 : P4;
+    float* to = a.partial + ((int64_t)blockIdx.x * 4 + k) * a.width;
+    if constexpr (ROWS == 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (in_row<E, LANES>(e, lane, a.width)) to[((e >> 2) * LANES + lane) * 4 + (e & 3)] = P[e];
+    } else {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < E; ++e) cols[(threadIdx.x / LANES) * (LANES * E) + ((e >> 2) * LANES + lane) * 4 + (e & 3)] = P[e];
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.width; c += THREADS) {
+        float s = 0.0f;
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) s += cols[r * (LANES * E) + c];
+        to[c] = s;
+      }
+    }
+  }
+}
+
+template <typename TX, typename TY, bool BACK, int LANES, int E>
+int residual_launch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
+  constexpr int THREADS = LANES > 256 ? LANES : 256;
+  if (a.width % 4) {
+    if (BACK) hipLaunchKernelGGL((k_residual_backward<TX, TY, LANES, E, true>), dim3(grid), dim3(THREADS), 0, stream, a);
+    else hipLaunchKernelGGL((k_residual_forward<TX, TY, LANES, E, true>), dim3(grid), dim3(THREADS), 0, stream, a);
+  } else {
+    if (BACK) hipLaunchKernelGGL((k_residual_backward<TX, TY, LANES, E, false>), dim3(grid), dim3(THREADS), 0, stream, a);
+    else hipLaunchKernelGGL((k_residual_forward<TX, TY, LANES, E, false>), dim3(grid), dim3(THREADS), 0, stream, a);
+  }
+  DISCO_CHECK_LAUNCH();
+  return DISCO_OK;
+}
+
+template <typename TX, typename TY, bool BACK>
+int residual_dispatch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
+  const ResidualShape s = residual_shape(a.width);
+  switch (s.lanes * 100 + s.elems) {
+    case 1604: return residual_launch<TX, TY, BACK, 16, 4>(a, grid, stream);
+    case 3204: return residual_launch<TX, TY, BACK, 32, 4>(a, grid, stream);
+    case 6404: return residual_launch<TX, TY, BACK, 64, 4>(a, grid, stream);
+    case 6408: return residual_launch<TX, TY, BACK, 64, 8>(a, grid, stream);
+    case 6412: return residual_launch<TX, TY, BACK, 64, 12>(a, grid, stream);
+    case 6416: return residual_launch<TX, TY, BACK, 64, 16>(a, grid, stream);
+    case 25608: return residual_launch<TX, TY, BACK, 256, 8>(a, grid, stream);
+    case 25616: return residual_launch<TX, TY, BACK, 256, 16>(a, grid, stream);
+    case 51216: return residual_launch<TX, TY, BACK, 512, 16>(a, grid, stream);
+    case 102416: return residual_launch<TX, TY, BACK, 1024, 16>(a, grid, stream);
+  }
+  return DISCO_EUNSUPPORTED;
+}
+
+#define DISCO_RESIDUAL_PAIR(PAIR, TX, TY)                                                                  \
+  namespace disco {                                                                                        \
+  template <> int residual_forward<PAIR>(const ResidualArgs& a, unsigned grid, hipStream_t stream) {        \
+    return residual_dispatch<TX, TY, false>(a, grid, stream);                                              \
+  }                                                                                                        \
+  template <> int residual_backward<PAIR>(const ResidualArgs& a, unsigned grid, hipStream_t stream) {       \
+    return residual_dispatch<TX, TY, true>(a, grid, stream);                                               \
+  }                                                                                                        \
+  }
+
+#endif  // DISCO_RESIDUAL_KERNELS
+
+}  // namespace disco
+#endif

@@ -1,0 +1,199 @@
+// disco_residual.hip -- C entries of the join between two residual blocks, and the end of its parameter gradients.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "disco_residual.h"
+
+namespace disco {
+
+__device__ __forceinline__ float param_at(const void* p, int type, int64_t i) {
+  if (type == DISCO_F32) return static_cast<const float*>(p)[i];
+  if (type == DISCO_F16) return (float)static_cast<const _Float16*>(p)[i];
+  return (float)static_cast<const __bf16*>(p)[i];
+}
+__device__ __forceinline__ void param_put(void* p, int type, int64_t i, double v) {
+  if (type == DISCO_F32) static_cast<float*>(p)[i] = (float)v;
+  else if (type == DISCO_F16) static_cast<_Float16*>(p)[i] = (_Float16)(float)v;
+  else static_cast<__bf16*>(p)[i] = (__bf16)(float)v;
+}
+
+struct FinishArgs {
+  const float* partial;
+  int64_t groups;
+  int width, partials, param_type, channel, act;
+  float scale;
+  const void *w1, *b1, *lam, *g;
+  void *dw1, *db1, *dw2, *db2, *dlam, *dg;
+};
+
+// Parameter gradients from the workgroups' column sums: 16 columns per workgroup, 64 lanes down each column, sums in
+// float64 in a fixed order.  With c = act(channel gate) and s the scale, z = u1 * w1 + b1 gives
+//   dw1 = s c P1,  db1 = s c P2,  ds = c (w1 P1 + b1 P2),  dgate = s c' (w1 P1 + b1 P2),  dw2 = P3,  db2 = P4.
+__global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
+  __shared__ double part[4][64][16];
+  const int cl = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int c = blockIdx.x * 16 + cl;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    double s = 0.0;
+    if (c < a.width && (a.partials >> k & 1))
+      for (int64_t g = slice; g < a.groups; g += 64) s += (double)a.partial[(g * 4 + k) * a.width + c];
+    part[k][slice][cl] = s;
+  }
+  __syncthreads();
+  for (int o = 32; o > 0; o >>= 1) {
+    if (slice < o)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) part[k][slice][cl] += part[k][slice + o][cl];
+    __syncthreads();
+  }
+  if (slice != 0 || c >= a.width) return;
+  const double P1 = part[0][0][cl], P2 = part[1][0][cl];
+  const double w = a.w1 ? (double)param_at(a.w1, a.param_type, c) : 1.0, b = a.b1 ? (double)param_at(a.b1, a.param_type, c) : 0.0;
+  const double s = (double)a.scale * (a.lam ? (double)param_at(a.lam, a.param_type, c) : 1.0);
+  double gate = 1.0, slope = 0.0;
+  if (a.channel) {
+    const double g = (double)param_at(a.g, a.param_type, c);
+    if (a.act == DISCO_ACT_SIGMOID) { gate = 1.0 / (1.0 + exp(-g)); slope = gate * (1.0 - gate); }
+    else if (a.act == DISCO_ACT_TANH) { gate = tanh(g); slope = 1.0 - gate * gate; }
+    else { gate = g; slope = 1.0; }
+  }
+  if (a.dw1) param_put(a.dw1, a.param_type, c, s * gate * P1);
+  if (a.db1) param_put(a.db1, a.param_type, c, s * gate * P2);
+  const double T = w * P1 + b * P2;
+  if (a.dlam) param_put(a.dlam, a.param_type, c, (double)a.scale * gate * T);
+  if (a.channel && a.dg) param_put(a.dg, a.param_type, c, s * slope * T);
+  if (a.dw2) param_put(a.dw2, a.param_type, c, part[2][0][cl]);
+  if (a.db2) param_put(a.db2, a.param_type, c, part[3][0][cl]);
+}
+
+static int pair_of(int stream_type, int block_type) {
+  if (stream_type == block_type) return stream_type == DISCO_F32 ? kPairF32 : stream_type == DISCO_F16 ? kPairF16 : stream_type == DISCO_BF16 ? kPairBF16 : -1;
+  if (stream_type == DISCO_F32) return block_type == DISCO_F16 ? kPairF32F16 : block_type == DISCO_BF16 ? kPairF32BF16 : -1;
+  return -1;
+}
+
+static int check_desc(const disco_residual_norm* d) {
+  if (!d || d->rows < 0 || d->width < 1 || !(d->eps > 0.0f) || !isfinite(d->eps)) return DISCO_EINVAL;
+  if (d->param_type < DISCO_F32 || d->param_type > DISCO_BF16 || pair_of(d->stream_type, d->block_type) < 0) return DISCO_EINVAL;
+  if (d->post_norm < DISCO_NORM_NONE || d->post_norm > DISCO_NORM_LAYER || d->pre_norm < DISCO_NORM_NONE || d->pre_norm > DISCO_NORM_LAYER)
+    return DISCO_EINVAL;
+  if (d->gate_kind < DISCO_GATE_NONE || d->gate_kind > DISCO_GATE_CHANNEL || d->gate_act < DISCO_ACT_NONE || d->gate_act > DISCO_ACT_TANH)
+    return DISCO_EINVAL;
+  if (!d->has_block && (d->post_norm || d->gate_kind || d->scale_vector || d->post_weight || d->post_bias || !d->pre_norm)) return DISCO_EINVAL;
+  if (!d->post_norm && (d->post_weight || d->post_bias)) return DISCO_EINVAL;
+  if (!d->pre_norm && (d->pre_weight || d->pre_bias)) return DISCO_EINVAL;
+  if (d->gate_kind == DISCO_GATE_CHANNEL && !d->gate) return DISCO_EINVAL;
+  if (d->width > DISCO_RESIDUAL_MAX_WIDTH) return DISCO_EUNSUPPORTED;
+  return DISCO_OK;
+}
+
+static void fill(const disco_residual_norm* d, ResidualArgs* a) {
+  *a = ResidualArgs{};
+  a->rows = d->rows; a->width = (int)d->width;
+  a->ldx = d->ldx; a->ldy = d->ldy; a->ldg = d->ld_gate;
+  a->param_type = d->param_type; a->post = d->post_norm; a->pre = d->pre_norm; a->gate = d->gate_kind; a->act = d->gate_act;
+  a->scale = d->scale; a->eps = d->eps; a->inv_width = 1.0f / (float)d->width;
+  a->x = d->x; a->y = d->has_block ? d->y : nullptr; a->g = d->gate;
+  a->w1 = d->post_weight; a->b1 = d->post_bias; a->w2 = d->pre_weight; a->b2 = d->pre_bias; a->lam = d->scale_vector;
+}
+
+static unsigned turns(int64_t rows, const ResidualShape& s, int64_t most) {
+  const int64_t at_a_time = s.threads / s.lanes, want = (rows + at_a_time - 1) / at_a_time;
+  return (unsigned)(want < most ? want : most);
+}
+// workgroups of a launch: every compute unit (256) can hold all of them at once, each walks its share of the rows
+static unsigned forward_grid(int64_t rows, const ResidualShape& s) { return turns(rows, s, 2048 * 256 / s.threads); }
+static unsigned backward_grid(int64_t rows, const ResidualShape& s) { return turns(rows, s, 1024 * 256 / s.threads); }
+
+static bool strided(int64_t ld, int64_t rows, int64_t width) { return rows <= 1 || ld >= width; }
+
+}  // namespace disco
+
+using namespace disco;
+
+extern "C" int disco_residual_norm_forward(const disco_residual_norm* d, void* out, int64_t ld_out, void* h, int64_t ld_h,
+                                           float* stats, void* stream_) {
+  const int rc = check_desc(d);
+  if (rc != DISCO_OK) return rc;
+  const int64_t n = d->rows, F = d->width;
+  if (!strided(ld_out, n, F) && d->has_block) return DISCO_EINVAL;
+  if (!strided(ld_h, n, F) && d->pre_norm) return DISCO_EINVAL;
+  if (n == 0) return DISCO_OK;
+  if (d->ldx < 0 || d->ldy < 0 || d->ld_gate < 0) return DISCO_EINVAL;
+  if (!d->x || (d->has_block && (!d->y || !out)) || (d->pre_norm && !h) || (d->gate_kind && !d->gate)) return DISCO_EINVAL;
+  ResidualArgs a;
+  fill(d, &a);
+  a.out = out; a.ldo = ld_out; a.h = h; a.ldh = ld_h; a.stats = stats;
+  const ResidualShape s = residual_shape(F);
+  const unsigned grid = forward_grid(n, s);
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  switch (pair_of(d->stream_type, d->block_type)) {
+    case kPairF32: return residual_forward<kPairF32>(a, grid, stream);
+    case kPairF16: return residual_forward<kPairF16>(a, grid, stream);
+    case kPairBF16: return residual_forward<kPairBF16>(a, grid, stream);
+    case kPairF32F16: return residual_forward<kPairF32F16>(a, grid, stream);
+    default: return residual_forward<kPairF32BF16>(a, grid, stream);
+  }
+}
+
+extern "C" size_t disco_residual_norm_workspace_bytes(int64_t rows, int64_t width) {
+  if (rows < 0 || width < 1 || width > DISCO_RESIDUAL_MAX_WIDTH) return 0;
+  return (size_t)backward_grid(rows, residual_shape(width)) * 4 * (size_t)width * sizeof(float);
+}
+
+extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const float* stats, const disco_residual_norm_grads* g,
+                                            void* workspace, size_t workspace_bytes, void* stream_) {
+  const int rc = check_desc(d);
+  if (rc != DISCO_OK) return rc;
+  if (!g) return DISCO_EINVAL;
+  const int64_t n = d->rows, F = d->width;
+  if (!d->has_block && (g->dy || g->dgate || g->dscale || g->dpost_weight || g->dpost_bias || g->dout)) return DISCO_EINVAL;
+  if ((g->dpost_weight && !d->post_weight) || (g->dpost_bias && !d->post_bias) || (g->dpre_weight && !d->pre_weight) ||
+      (g->dpre_bias && !d->pre_bias) || (g->dscale && !d->scale_vector) || (g->dgate && !d->gate_kind) || (g->dh && !d->pre_norm))
+    return DISCO_EINVAL;
+  ResidualArgs a;
+  fill(d, &a);
+  const bool channel = d->gate_kind == DISCO_GATE_CHANNEL;
+  const bool branch = g->dscale || (channel && g->dgate);
+  a.partials = (g->dpost_weight || branch ? 1 : 0) | (g->dpost_bias || (branch && d->post_bias) ? 2 : 0) | (g->dpre_weight ? 4 : 0) |
+               (g->dpre_bias ? 8 : 0);
+  if (n > 0) {
+    if (!strided(g->ld_dx, n, F) || !strided(g->ld_dy, n, F) || (d->gate_kind == DISCO_GATE_FULL && g->dgate && !strided(g->ld_dgate, n, F)) ||
+        (d->gate_kind == DISCO_GATE_ROW && g->dgate && g->ld_dgate < 1 && n > 1))
+      return DISCO_EINVAL;
+    if (d->ldx < 0 || d->ldy < 0 || d->ld_gate < 0 || g->ld_dout < 0 || g->ld_dh < 0) return DISCO_EINVAL;
+    if ((d->has_block && !d->y) || (g->dh && !d->x) || (d->gate_kind && !d->gate) || ((d->post_norm || g->dh) && !stats)) return DISCO_EINVAL;
+  }
+  const ResidualShape s = residual_shape(F);
+  const unsigned grid = backward_grid(n, s);
+  const size_t need = (size_t)grid * 4 * (size_t)F * sizeof(float);
+  if (a.partials && n > 0 && (!workspace || workspace_bytes < need)) return DISCO_EWORKSPACE;
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  a.stats = const_cast<float*>(stats);
+  a.dout = g->dout; a.lddo = g->ld_dout; a.dh = g->dh; a.lddh = g->ld_dh;
+  a.dx = g->dx; a.lddx = g->ld_dx; a.dy = g->dy; a.lddy = g->ld_dy; a.dg = channel ? nullptr : g->dgate; a.lddg = g->ld_dgate;
+  a.partial = a.partials ? static_cast<float*>(workspace) : nullptr;
+  if (n > 0) {
+    int r;
+    switch (pair_of(d->stream_type, d->block_type)) {
+      case kPairF32: r = residual_backward<kPairF32>(a, grid, stream); break;
+      case kPairF16: r = residual_backward<kPairF16>(a, grid, stream); break;
+      case kPairBF16: r = residual_backward<kPairBF16>(a, grid, stream); break;
+      case kPairF32F16: r = residual_backward<kPairF32F16>(a, grid, stream); break;
+      default: r = residual_backward<kPairF32BF16>(a, grid, stream);
+    }
+    if (r != DISCO_OK) return r;
+  }
+  if (!a.partials) return DISCO_OK;
+  FinishArgs f{};
+  f.partial = a.partial; f.groups = n > 0 ? grid : 0; f.width = (int)F; f.partials = a.partials; f.param_type = d->param_type;
+  f.channel = channel; f.act = d->gate_act; f.scale = d->scale;
+  f.w1 = d->post_weight; f.b1 = d->post_bias; f.lam = d->scale_vector; f.g = channel ? d->gate : nullptr;
+  f.dw1 = g->dpost_weight; f.db1 = g->dpost_bias; f.dw2 = g->dpre_weight; f.db2 = g->dpre_bias; f.dlam = g->dscale;
+  f.dg = channel ? g->dgate : nullptr;
+  hipLaunchKernelGGL(k_residual_finish, dim3((unsigned)((F + 15) / 16)), dim3(1024), 0, stream, f);
+  DISCO_CHECK_LAUNCH();
+  return DISCO_OK;
+}

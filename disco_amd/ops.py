@@ -5,6 +5,8 @@ spmm       <- torch_sparse.matmul(adj_t, x, reduce)      sg_conv.py:92-93, gcn_c
 khop       <- for k in range(K): x = propagate(adj_t, x)  sg_conv.py:74-77
 max_aggregate <- MessagePassing(aggr="max").propagate     LargeScaleCondensing.py:152-172
 anchor_max <- feat_transform[index[c]][anchor, :L*d].max(dim=1).values   LargeScaleCondensing.py:299
+residual_norm / row_norm        norms before and after a residual block, its gate and scale    (residual.py)
+grad_norm / clip_grads          the norm over all gradients of a model, and clipping           (gradients.py)
 (paths relative to /root/reference)
 """
 from __future__ import annotations
@@ -14,6 +16,8 @@ from typing import Optional
 import torch
 
 from . import _lib
+from .gradients import clip_grad_norm_, clip_grads, grad_norm  # noqa: F401
+from .residual import residual_norm, row_norm  # noqa: F401
 from .sparse import SparseTensor
 
 _REDUCE = {"sum": 0, "add": 0, "mean": 1, "max": 2, "sum_acc": 3}

@@ -357,6 +357,71 @@ int disco_anchor_max_f32(const float* T, int64_t n, int64_t ldt, int64_t width, 
                          const int64_t* anchor, int64_t n_out, int64_t k, const int64_t* out_rows, int64_t n_dst,
                          float* out, int64_t ldo, int* err_flag, void* stream);
 
+/* ---- The join between two residual blocks: norms, gate, scale and residual sum in one pass ----------------
+ *   z   = N_post(y)                      the block's output, normalised (DISCO_NORM_NONE: as it is)
+ *   out = x + scale * scale_vector * act(gate) * z
+ *   h   = N_pre(out)                     the next block's input (of the sum before it is rounded to x's type)
+ *   N_rms(v)   = v / sqrt(mean(v^2) + eps) * weight + bias
+ *   N_layer(v) = (v - mean(v)) / sqrt(mean((v - mean(v))^2) + eps) * weight + bias        (weight / bias NULL: 1 / 0)
+ * has_block = 0 leaves y, the gate and `out` away: h = N_pre(x), the norm before the first block.
+ * Rows are `width` elements at a leading dimension in elements (0 is allowed where only read: one row for all); columns
+ * have unit stride and rows need no alignment beyond their element's.  gate: [rows, width] (FULL, block type), [rows]
+ * at ld_gate (ROW, block type) or [width] (CHANNEL, parameter type).  Types: stream_type of x, out and their gradients,
+ * block_type of y, h, gate and theirs -- equal, or float32 with a 16-bit block -- and param_type of every vector.
+ * Statistics and sums are float32 or float64; values are rounded to their type once.  A NaN or infinity stays in its row
+ * (and in the parameter gradients).  No counterpart in the reference, which normalises hidden layers with stock BatchNorm
+ * (/root/reference/models/basicgnn_large.py:119-133) and has no residual blocks. */
+enum disco_dtype { DISCO_F32 = 0, DISCO_F16 = 1, DISCO_BF16 = 2 };
+enum disco_norm_kind { DISCO_NORM_NONE = 0, DISCO_NORM_RMS = 1, DISCO_NORM_LAYER = 2 };
+enum disco_gate_kind { DISCO_GATE_NONE = 0, DISCO_GATE_FULL = 1, DISCO_GATE_ROW = 2, DISCO_GATE_CHANNEL = 3 };
+enum disco_gate_act { DISCO_ACT_NONE = 0, DISCO_ACT_SIGMOID = 1, DISCO_ACT_TANH = 2 };
+#define DISCO_RESIDUAL_MAX_WIDTH 16384
+
+typedef struct disco_residual_norm {
+  int64_t rows, width, ldx, ldy, ld_gate;
+  const void *x, *y, *gate;
+  const void *post_weight, *post_bias, *pre_weight, *pre_bias, *scale_vector; /* [width] each, NULL: absent */
+  int32_t stream_type, block_type, param_type; /* disco_dtype */
+  int32_t has_block, post_norm, pre_norm;      /* disco_norm_kind */
+  int32_t gate_kind, gate_act;
+  float scale, eps; /* eps > 0 */
+} disco_residual_norm;
+
+/* Gradients of the outputs (NULL: zero) and of the inputs (NULL: not wanted; a gradient of an input that the descriptor
+ * leaves away is refused).  dgate has the gate's shape; the vectors' gradients have the parameter type. */
+typedef struct disco_residual_norm_grads {
+  const void *dout, *dh;
+  void *dx, *dy, *dgate;
+  int64_t ld_dout, ld_dh, ld_dx, ld_dy, ld_dgate;
+  void *dpost_weight, *dpost_bias, *dpre_weight, *dpre_bias, *dscale;
+} disco_residual_norm_grads;
+
+/* `stats` (float32 [4 * rows], may be NULL where no backward follows) keeps the rows' means and inverse deviations.  The
+ * backward takes the forward's descriptor and stats, reads x (where dh is given), y and gate again and sums the vectors'
+ * gradients in a fixed order through `workspace`.  Widths above DISCO_RESIDUAL_MAX_WIDTH: DISCO_EUNSUPPORTED. */
+int disco_residual_norm_forward(const disco_residual_norm* desc_host, void* out, int64_t ld_out, void* h, int64_t ld_h,
+                                float* stats, void* stream);
+size_t disco_residual_norm_workspace_bytes(int64_t rows, int64_t width);
+int disco_residual_norm_backward(const disco_residual_norm* desc_host, const float* stats,
+                                 const disco_residual_norm_grads* grads_host, void* workspace, size_t workspace_bytes,
+                                 void* stream);
+
+/* ---- Norm over all gradients of a model, and clipping ------------------------------------------------------
+ *   norm = (sum |g|^p)^(1/p) over every element of every tensor; norm_type p = 1, 2, or 0 for the largest |g|
+ *   out  = g * min(1, max_norm / (norm + 1e-6))
+ * The arrays named `_host` have n_tensors entries in host memory (device pointers, element counts, disco_dtype) and are
+ * read before the call returns: nothing is copied to the device, a call can be captured.  Each tensor is contiguous.  An
+ * output has its gradient's type or float32, may be the gradient itself (in place), and overlaps nothing else
+ * (DISCO_EINVAL).  `norm` is one device float.  Sums are float64 in a fixed order.  A norm that is infinite scales by
+ * zero (infinite entries become NaN), one that is NaN makes every output NaN.  Gradients in place within max_norm are not
+ * written.  No counterpart in the reference, whose training loops do not clip (LargeScaleCondensing.py:187-200). */
+size_t disco_grad_norm_workspace_bytes(int64_t n_tensors);
+int disco_grad_norm(const void* const* grads_host, const int64_t* numel_host, const int* type_host, int64_t n_tensors,
+                    int norm_type, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+int disco_grad_clip(const void* const* grads_host, void* const* out_host, const int64_t* numel_host, const int* type_host,
+                    const int* out_type_host, int64_t n_tensors, int norm_type, double max_norm, float* norm,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

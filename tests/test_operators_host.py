@@ -1,0 +1,155 @@
+"""Refusals of the residual join, the row norm and the gradient norm that need no GPU: arguments are checked before the
+device is touched, in Python and again at the C entries."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from disco_amd import _lib, ops
+
+F, N = 12, 5
+
+
+def _xy(dtype=torch.float32, block=None):
+    return torch.zeros(N, F, dtype=dtype), torch.zeros(N, F, dtype=block or dtype)
+
+
+@pytest.mark.parametrize("kwargs,error", [
+    (dict(post="batch"), ValueError), (dict(pre="batch"), ValueError), (dict(gate=torch.zeros(F), gate_act="relu"), ValueError),
+    (dict(gate_act="sigmoid"), ValueError), (dict(gate=torch.zeros(N)), ValueError), (dict(gate=torch.zeros(N, 2)), ValueError),
+    (dict(gate=torch.zeros(1, F)), ValueError), (dict(gate=torch.zeros(N, F, dtype=torch.float16)), TypeError),
+    (dict(gate=torch.zeros(N, 1, dtype=torch.bfloat16)), TypeError), (dict(gate=torch.zeros(F, dtype=torch.float64)), TypeError),
+    (dict(scale=math.nan), ValueError), (dict(scale=math.inf), ValueError), (dict(scale=torch.zeros(F + 1)), ValueError),
+    (dict(scale=torch.zeros(())), ValueError), (dict(scale=torch.zeros(F, dtype=torch.int64)), TypeError),
+    (dict(post_weight=torch.ones(F)), ValueError), (dict(post_bias=torch.ones(F)), ValueError),
+    (dict(pre_weight=torch.ones(F)), ValueError), (dict(pre_bias=torch.ones(F)), ValueError),
+    (dict(pre="rms", pre_weight=torch.ones(F, 1)), ValueError), (dict(post="rms", post_weight=torch.ones(F).double()), TypeError),
+    (dict(eps=0.0), ValueError), (dict(eps=-1e-5), ValueError), (dict(eps=math.nan), ValueError), (dict(eps=math.inf), ValueError),
+    (dict(), RuntimeError),                       # all in order, but on the CPU
+    (dict(pre="layer", post="rms", gate=torch.zeros(N, 1), gate_act="tanh", scale=torch.ones(F)), RuntimeError)])
+def test_residual_norm_refuses(kwargs, error):
+    with pytest.raises(error):
+        ops.residual_norm(*_xy(), **kwargs)
+
+
+@pytest.mark.parametrize("x,y,error", [
+    (torch.zeros(N, F), torch.zeros(N, F + 1), ValueError), (torch.zeros(N, F), torch.zeros(N + 1, F), ValueError),
+    (torch.zeros(F), torch.zeros(F), ValueError), (torch.zeros(2, N, F), torch.zeros(2, N, F), ValueError),
+    (torch.zeros(N, 0), torch.zeros(N, 0), ValueError), (torch.zeros(1, 16385), torch.zeros(1, 16385), ValueError),
+    (torch.zeros(N, F).double(), torch.zeros(N, F).double(), TypeError), (torch.zeros(N, F).half(), torch.zeros(N, F), TypeError),
+    (torch.zeros(N, F).half(), torch.zeros(N, F).bfloat16(), TypeError), (torch.zeros(N, F), torch.zeros(N, F).double(), TypeError),
+    (torch.zeros(N, F), None, TypeError), (torch.zeros(N, F).to_sparse(), torch.zeros(N, F), TypeError)])
+def test_residual_norm_refuses_operands(x, y, error):
+    with pytest.raises(error):
+        ops.residual_norm(x, y)
+
+
+@pytest.mark.parametrize("args,kwargs,error", [
+    ((), dict(kind="batch"), ValueError), ((), dict(kind=None), ValueError), ((torch.ones(F + 1),), {}, ValueError),
+    ((torch.ones(F), torch.ones(2)), {}, ValueError), ((), dict(eps=0.0), ValueError), ((), dict(dtype=torch.float64), TypeError),
+    ((), {}, RuntimeError), ((), dict(dtype=torch.bfloat16), RuntimeError)])
+def test_row_norm_refuses(args, kwargs, error):
+    with pytest.raises(error):
+        ops.row_norm(torch.zeros(N, F), *args, **kwargs)
+    with pytest.raises(TypeError):
+        ops.row_norm(torch.zeros(N, F).half(), dtype=torch.float32)
+
+
+def test_gradient_norm_refuses():
+    g = [torch.zeros(3), torch.zeros(2, 2)]
+    for p in (3, 0, -1, 0.5, math.nan):
+        with pytest.raises(ValueError):
+            ops.grad_norm(g, p)
+    with pytest.raises(TypeError):
+        ops.grad_norm([torch.zeros(3).double()])
+    with pytest.raises(TypeError):
+        ops.grad_norm([torch.zeros(3, 3).to_sparse()])
+    with pytest.raises(TypeError):
+        ops.grad_norm([None])
+    with pytest.raises(ValueError):
+        ops.grad_norm([torch.zeros(3), torch.zeros(3, device="meta")])
+    for bad in (-1.0, math.nan, -math.inf):
+        with pytest.raises(ValueError):
+            ops.clip_grads(g, bad)
+    for out in ([torch.zeros(3)], [torch.zeros(3), torch.zeros(4)], [torch.zeros(3), torch.zeros(2, 2).half()]):
+        with pytest.raises(ValueError):
+            ops.clip_grads(g, 1.0, out=out)
+    for call in (lambda: ops.grad_norm(g), lambda: ops.clip_grads(g, 1.0), lambda: ops.clip_grads(g, 1.0, out=[t.clone() for t in g])):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            call()
+
+
+def _desc(**k):
+    base = dict(rows=4, width=8, ldx=8, ldy=8, ld_gate=8, x=64, y=64, has_block=1, eps=1e-5, scale=1.0)
+    return _lib.ResidualNorm(**{**base, **k})
+
+
+@pytest.mark.parametrize("change", [
+    dict(rows=-1), dict(width=0), dict(width=-3), dict(eps=0.0), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf),
+    dict(stream_type=3), dict(block_type=3), dict(stream_type=1), dict(stream_type=1, block_type=2), dict(param_type=-1),
+    dict(post_norm=3), dict(pre_norm=-1), dict(gate_kind=4), dict(gate_act=3), dict(x=None), dict(y=None), dict(gate_kind=1),
+    dict(gate_kind=2), dict(gate_kind=3), dict(post_weight=64), dict(pre_bias=64), dict(ldx=-1), dict(ldy=-8),
+    dict(has_block=0), dict(has_block=0, pre_norm=1, post_norm=1), dict(has_block=0, pre_norm=1, scale_vector=64),
+    dict(has_block=0, pre_norm=1, gate_kind=1, gate=64)])
+def test_residual_entries_refuse(change):
+    lib = _lib.load()
+    d = _desc(**change)
+    assert lib.disco_residual_norm_forward(d, 64, 8, 64, 8, None, None) == -1
+    g = _lib.ResidualNormGrads(dx=64, ld_dx=8, ld_dy=8, ld_dgate=8)
+    if change.get("x", 64) is not None:           # the backward reads x only for the gradient of h
+        assert lib.disco_residual_norm_backward(d, 64, g, 64, 1 << 20, None) == -1
+
+
+def test_residual_entries_refuse_more():
+    lib = _lib.load()
+    assert lib.disco_residual_norm_forward(None, 64, 8, 64, 8, None, None) == -1
+    assert lib.disco_residual_norm_forward(_desc(), None, 8, None, 8, None, None) == -1          # out is missing
+    assert lib.disco_residual_norm_forward(_desc(pre_norm=1), 64, 8, None, 8, None, None) == -1  # h is missing
+    assert lib.disco_residual_norm_forward(_desc(), 64, 7, None, 8, None, None) == -1            # rows of out overlap
+    assert lib.disco_residual_norm_forward(_desc(width=16385), 64, 16385, None, 8, None, None) == -2
+    assert lib.disco_residual_norm_forward(_desc(rows=0, x=None, y=None), None, 8, None, 8, None, None) == 0
+    assert lib.disco_residual_norm_backward(_desc(), None, None, None, 0, None) == -1
+    G = _lib.ResidualNormGrads
+    ld = dict(ld_dx=8, ld_dy=8, ld_dgate=8)
+    for d, g in ((_desc(), G(dpost_weight=64, **ld)), (_desc(), G(dpre_bias=64, **ld)), (_desc(), G(dscale=64, **ld)),
+                 (_desc(), G(dgate=64, **ld)), (_desc(), G(dh=64, **ld)), (_desc(), G(dx=64, ld_dx=3, ld_dy=8, ld_dgate=8)),
+                 (_desc(has_block=0, pre_norm=1), G(dy=64, **ld)), (_desc(has_block=0, pre_norm=1), G(dout=64, **ld)),
+                 (_desc(gate_kind=2, gate=64, ld_gate=1), G(dgate=64, ld_dx=8, ld_dy=8, ld_dgate=0))):
+        assert lib.disco_residual_norm_backward(d, 64, g, 64, 1 << 20, None) == -1
+    d = _desc(pre_norm=1, pre_weight=64)
+    assert lib.disco_residual_norm_backward(d, None, G(dh=64, dx=64, ld_dh=8, **ld), None, 0, None) == -1        # stats are missing
+    assert lib.disco_residual_norm_backward(d, 64, G(dh=64, dpre_weight=64, ld_dh=8, **ld), None, 0, None) == -3
+    need = lib.disco_residual_norm_workspace_bytes(4, 8)
+    assert need > 0 and lib.disco_residual_norm_backward(d, 64, G(dh=64, dpre_weight=64, ld_dh=8, **ld), 64, need - 1, None) == -3
+    for rows, width in ((-1, 8), (4, 0), (4, 16385)):
+        assert lib.disco_residual_norm_workspace_bytes(rows, width) == 0
+
+
+def test_gradient_entries_refuse():
+    lib = _lib.load()
+    ws = lib.disco_grad_norm_workspace_bytes(2)
+    assert ws > 0 and lib.disco_grad_norm_workspace_bytes(-1) == 0
+
+    def norm(ptrs=(4096, 8192), numel=(10, 10), types=(0, 0), n=2, p=2, out=64, work=64, nb=ws):
+        return lib.disco_grad_norm((C.c_void_p * 2)(*ptrs), (C.c_int64 * 2)(*numel), (C.c_int * 2)(*types), n, p, out, work, nb, None)
+
+    assert norm(ptrs=(None, 8192)) == -1 and norm(numel=(-1, 3)) == -1 and norm(types=(0, 3)) == -1 and norm(n=-1) == -1
+    assert norm(p=3) == -1 and norm(p=-1) == -1 and norm(out=None) == -1 and norm(work=None) == -1 and norm(nb=8) == -3
+    assert lib.disco_grad_norm(None, None, None, 2, 2, 64, 64, ws, None) == -1
+
+    def clip(src=(4096, 8192), dst=(4096, 8192), numel=(10, 10), types=(0, 0), to=(0, 0), p=2, most=1.0, out=64, work=64, nb=8):
+        return lib.disco_grad_clip((C.c_void_p * 2)(*src), (C.c_void_p * 2)(*dst), (C.c_int64 * 2)(*numel), (C.c_int * 2)(*types),
+                                   (C.c_int * 2)(*to), 2, p, most, out, work, nb, None)
+
+    assert clip() == -3                                                    # all in order, the workspace is too small
+    assert clip(most=-1.0) == -1 and clip(most=math.nan) == -1 and clip(p=7) == -1 and clip(out=None) == -1 and clip(work=None) == -1
+    assert clip(to=(1, 0)) == -1 and clip(types=(1, 1), to=(2, 2)) == -1   # neither the gradient's type nor float32
+    assert clip(dst=(None, 8192)) == -1
+    # shared memory: the same tensor twice, a part of another, an output over another gradient, over its own with an offset
+    assert clip(src=(4096, 4096), dst=(4096, 4096)) == -1
+    assert clip(src=(4096, 4132), dst=(4096, 4132)) == -1
+    assert clip(src=(4096, 4136), dst=(4096, 4136)) == -3
+    assert clip(dst=(8192, 4096)) == -1 and clip(dst=(4100, 8192)) == -1
+    assert clip(types=(1, 1), to=(0, 1)) == -1                             # in place with a wider type
+    assert clip(src=(4096, 4096), dst=(16384, 32768)) == -3                # read twice, written apart: allowed
