@@ -37,14 +37,17 @@ struct ResidualArgs {
 
 enum ResidualPair { kPairF32 = 0, kPairF16 = 1, kPairBF16 = 2, kPairF32F16 = 3, kPairF32BF16 = 4 };
 
-// A kernel variant: lanes per row and elements a lane holds; the workgroup has 256 lanes, or a row's if those are more.
-struct ResidualShape { int lanes, elems, threads; };
+// A kernel variant: lanes per row and elements a lane holds.
+struct ResidualShape { int lanes, elems; };
 inline ResidualShape residual_shape(int64_t width) {
   const int table[][2] = {{16, 4}, {32, 4}, {64, 4}, {64, 8}, {64, 12}, {64, 16}, {256, 8}, {256, 16}, {512, 16}, {1024, 16}};
   for (const auto& t : table)
-    if (width <= (int64_t)t[0] * t[1]) return {t[0], t[1], t[0] > 256 ? t[0] : 256};
-  return {0, 0, 0};
+    if (width <= (int64_t)t[0] * t[1]) return {t[0], t[1]};
+  return {0, 0};
 }
+
+// lanes of a workgroup of the backward (see there)
+constexpr int residual_back_threads(int lanes, int elems) { return lanes > 64 ? lanes : elems <= 8 ? 1024 : elems <= 12 ? 768 : 512; }
 
 // grid: workgroups; a workgroup takes rows / (its rows at a time * grid) turns
 template <int PAIR> int residual_forward(const ResidualArgs& a, unsigned grid, hipStream_t stream);
@@ -56,12 +59,6 @@ template <int T> struct TypeOf;
 template <> struct TypeOf<DISCO_F32> { typedef float type; };
 template <> struct TypeOf<DISCO_F16> { typedef _Float16 type; };
 template <> struct TypeOf<DISCO_BF16> { typedef __bf16 type; };
-
-__device__ __forceinline__ float load_param(const void* p, int type, int64_t i) {
-  if (type == DISCO_F32) return static_cast<const float*>(p)[i];
-  if (type == DISCO_F16) return (float)static_cast<const _Float16*>(p)[i];
-  return (float)static_cast<const __bf16*>(p)[i];
-}
 
 __device__ __forceinline__ float activate(float g, int act) {
   if (act == DISCO_ACT_SIGMOID) return 1.0f / (1.0f + expf(-g));
@@ -113,30 +110,55 @@ struct RowPart {
   }
 };
 
+// Adds the value of a partner lane: within 16 lanes through the adder's own lane permutations, beyond through the row and
+// half swaps (both results of a swap of a value with itself add up to the pair's sum).  Every lane of a pair adds the same
+// two numbers, so all lanes of a row end with the same bits.  (Shuffles through LDS cost about 100 cycles a step, six steps a
+// sum and up to three sums a row: with them the trained join of 25000 x 602 took 216 us instead of 165 us.)
+template <int CTRL> __device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float add_swap16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_swap32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // Sums R values over the lanes of a row, the same in every lane.  The order is fixed: results do not vary from run to run.
 template <int LANES, int R>
-__device__ __forceinline__ void row_sum(float (&v)[R], float* lds, int& turn) {
-  constexpr int IN_WAVE = LANES < 64 ? LANES : 64;
+__device__ __forceinline__ void row_sum(float (&v)[R], float4* lds, int& turn) {
 #pragma unroll
-  for (int o = IN_WAVE / 2; o > 0; o >>= 1)
+  for (int r = 0; r < R; ++r) v[r] = add_dpp<0xB1>(v[r]);       // quad_perm [1, 0, 3, 2]
 #pragma unroll
-    for (int r = 0; r < R; ++r) v[r] += __shfl_xor(v[r], o, 64);
+  for (int r = 0; r < R; ++r) v[r] = add_dpp<0x4E>(v[r]);       // quad_perm [2, 3, 0, 1]
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = add_dpp<0x141>(v[r]);      // row_half_mirror
+#pragma unroll
+  for (int r = 0; r < R; ++r) v[r] = add_dpp<0x140>(v[r]);      // row_mirror
+  if constexpr (LANES >= 32)
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = add_swap16(v[r]);
+  if constexpr (LANES >= 64)
+#pragma unroll
+    for (int r = 0; r < R; ++r) v[r] = add_swap32(v[r]);
   if constexpr (LANES > 64) {
     constexpr int WAVES = LANES / 64;
     // two buffers in turn: a wave that is ahead by one reduction writes the other one, and cannot be ahead by two
-    float* part = lds + turn * (WAVES * 4);
+    float4* part = lds + turn * WAVES;
     turn ^= 1;
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-      for (int r = 0; r < R; ++r) part[(threadIdx.x >> 6) * 4 + r] = v[r];
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_float4(v[0], R > 1 ? v[R > 1 ? 1 : 0] : 0.0f, R > 2 ? v[R > 2 ? 2 : 0] : 0.0f, 0.0f);
     __syncthreads();
+    float4 s = part[0];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      float s = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) s += part[w * 4 + r];
-      v[r] = s;
+    for (int w = 1; w < WAVES; ++w) {
+      const float4 t = part[w];
+      s.x += t.x; s.y += t.y; s.z += t.z;
     }
+    v[0] = s.x;
+    if constexpr (R > 1) v[1] = s.y;
+    if constexpr (R > 2) v[2] = s.z;
   }
 }
 
@@ -146,7 +168,7 @@ __device__ __forceinline__ bool in_row(int e, int lane, int width) { return ((e 
 // Standardises a row in place and returns (mean, 1 / deviation).  The variance is summed from the deviations, after the
 // mean: subtracting two large sums would lose it.  Elements behind the width stay zero.
 template <int LANES, int E>
-__device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, float inv_width, int lane, int width, float* lds,
+__device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, float inv_width, int lane, int width, float4* lds,
                                             int& turn, float& mean, float& rstd) {
   float s[1] = {0.0f};
   mean = 0.0f;
@@ -167,43 +189,49 @@ __device__ __forceinline__ void standardise(float (&v)[E], int kind, float eps, 
   for (int e = 0; e < E; ++e) v[e] *= rstd;
 }
 
-// z = u1 * A + B with the residual scale and a channel gate folded in (A = lam * w1, B = lam * b1): loaded once per workgroup.
-template <int LANES, int E>
-__device__ __forceinline__ void load_branch(const ResidualArgs& a, int lane, float (&A)[E], float (&B)[E]) {
+// A parameter vector, `other` where it is absent; zero behind the width.
+template <int LANES, int E, bool ODD>
+__device__ __forceinline__ void load_vector(const void* p, int type, int lane, int width, float other, float (&v)[E]) {
+  if (!p) {
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int c = ((e >> 2) * LANES + lane) * 4 + (e & 3);
-    float lam = a.scale;
-    A[e] = B[e] = 0.0f;
-    if (c < a.width) {
-      if (a.lam) lam *= load_param(a.lam, a.param_type, c);
-      if (a.gate == DISCO_GATE_CHANNEL) lam *= activate(load_param(a.g, a.param_type, c), a.act);
-      A[e] = a.w1 ? lam * load_param(a.w1, a.param_type, c) : lam;
-      if (a.b1) B[e] = lam * load_param(a.b1, a.param_type, c);
-    }
+    for (int e = 0; e < E; ++e) v[e] = other;
+  } else if (type == DISCO_F32) {
+    RowPart<float, LANES, E, ODD>::load(v, static_cast<const float*>(p), lane, width);
+  } else if (type == DISCO_F16) {
+    RowPart<_Float16, LANES, E, ODD>::load(v, static_cast<const _Float16*>(p), lane, width);
+  } else {
+    RowPart<__bf16, LANES, E, ODD>::load(v, static_cast<const __bf16*>(p), lane, width);
   }
 }
 
-template <int LANES, int E>
-__device__ __forceinline__ void load_vector(const void* p, int type, int lane, int width, float other, float (&v)[E]) {
+// z = u1 * A + B with the residual scale and a channel gate folded in (A = lam * w1, B = lam * b1): loaded once per workgroup.
+template <int LANES, int E, bool ODD>
+__device__ __forceinline__ void load_branch(const ResidualArgs& a, int lane, float (&A)[E], float (&B)[E]) {
+  float g[E], lam[E];
+  load_vector<LANES, E, ODD>(a.w1, a.param_type, lane, a.width, 1.0f, A);
+  load_vector<LANES, E, ODD>(a.b1, a.param_type, lane, a.width, 0.0f, B);
+  load_vector<LANES, E, ODD>(a.lam, a.param_type, lane, a.width, 1.0f, lam);
+  load_vector<LANES, E, ODD>(a.gate == DISCO_GATE_CHANNEL ? a.g : nullptr, a.param_type, lane, a.width, 1.0f, g);
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const int c = ((e >> 2) * LANES + lane) * 4 + (e & 3);
-    v[e] = p && c < width ? load_param(p, type, c) : other;
+    float l = a.scale * lam[e];
+    if (a.gate == DISCO_GATE_CHANNEL) l *= activate(g[e], a.act);
+    A[e] *= l;
+    B[e] *= l;
   }
 }
 
 template <typename TX, typename TY, int LANES, int E, bool ODD>
 __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_forward(const ResidualArgs a) {
   constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
-  __shared__ float lds[2 * (THREADS / 64) * 4];
+  __shared__ float4 lds[LANES > 64 ? 2 * (LANES / 64) : 1];
   const int lane = threadIdx.x % LANES;
   int turn = 0;
   float A[E], B[E], W2[E], B2[E];
-  if (a.y) load_branch<LANES, E>(a, lane, A, B);
+  if (a.y) load_branch<LANES, E, ODD>(a, lane, A, B);
   if (a.pre) {
-    load_vector<LANES, E>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
-    load_vector<LANES, E>(a.b2, a.param_type, lane, a.width, 0.0f, B2);
+    load_vector<LANES, E, ODD>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
+    load_vector<LANES, E, ODD>(a.b2, a.param_type, lane, a.width, 0.0f, B2);
   }
   for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
     float o[E];
@@ -237,19 +265,56 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_forward(
   }
 }
 
+// The backward holds a row's x, y, gate and both gradients and four running column sums per element.  The three parameter
+// vectors that every row needs again stay in LDS (12 bytes an element beside the 20 to 32 that the row moves through memory):
+// in registers they cost a third of the waves that a compute unit can hold.  Rows of a wave or less share a workgroup as
+// large as the registers allow, since each workgroup leaves one partial row per sum behind for the finish to read.
 template <typename TX, typename TY, int LANES, int E, bool ODD>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward(const ResidualArgs a) {
-  constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
-  __shared__ float lds[2 * (THREADS / 64) * 4];
-  __shared__ float cols[ROWS > 1 ? THREADS * E : 1];
+__global__ __launch_bounds__(residual_back_threads(LANES, E), LANES < 1024 && E > 12 ? 2 : LANES == 256 ? 4 : 1) void k_residual_backward(const ResidualArgs a) {
+  constexpr int THREADS = residual_back_threads(LANES, E), ROWS = THREADS / LANES, W = LANES * E;
+  __shared__ float4 lds[LANES > 64 ? 2 * (LANES / 64) : 1];
+  // the vectors; after the last row, for rows of a wave or less, the column sums of the workgroup's row groups
+  __shared__ float4 store[(W <= 8192 ? (ROWS > 3 ? ROWS : 3) * W : 4) / 4];
+  constexpr bool IN_LDS = W <= 8192;
   const int lane = threadIdx.x % LANES;
   int turn = 0;
-  float A[E], B[E], W2[E], P1[E], P2[E], P3[E], P4[E];
-  if (a.y) load_branch<LANES, E>(a, lane, A, B);
-  if (a.pre) load_vector<LANES, E>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
+  float regs[IN_LDS ? 1 : 3][E], P1[E], P2[E], P3[E], P4[E];
+  {
+    float A[E], B[E], W2[E];
+    if (!IN_LDS || threadIdx.x < LANES) {
+      load_branch<LANES, E, ODD>(a, lane, A, B);
+      load_vector<LANES, E, ODD>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
+    }
+    if constexpr (IN_LDS) {
+      if (threadIdx.x < LANES)
+#pragma unroll
+        for (int k = 0; k < E / 4; ++k) {
+          store[k * LANES + lane] = make_float4(A[4 * k], A[4 * k + 1], A[4 * k + 2], A[4 * k + 3]);
+          store[W / 4 + k * LANES + lane] = make_float4(B[4 * k], B[4 * k + 1], B[4 * k + 2], B[4 * k + 3]);
+          store[W / 2 + k * LANES + lane] = make_float4(W2[4 * k], W2[4 * k + 1], W2[4 * k + 2], W2[4 * k + 3]);
+        }
+      __syncthreads();
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) { regs[0][e] = A[e]; regs[1][e] = B[e]; regs[2][e] = W2[e]; }
+    }
+  }
+  const auto vector = [&](int which, float (&v)[E]) {
+    if constexpr (IN_LDS) {
+#pragma unroll
+      for (int k = 0; k < E / 4; ++k) {
+        const float4 t = store[which * (W / 4) + k * LANES + lane];
+        v[4 * k] = t.x; v[4 * k + 1] = t.y; v[4 * k + 2] = t.z; v[4 * k + 3] = t.w;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = regs[which][e];
+    }
+  };
 #pragma unroll
   for (int e = 0; e < E; ++e) P1[e] = P2[e] = P3[e] = P4[e] = 0.0f;
   for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
+    if constexpr (IN_LDS) asm volatile("" ::: "memory");      // the vectors are read again, not kept in registers
     float u1[E], act[E], d[E], r1 = 1.0f, grow = 1.0f;
     if (a.y) {
       RowPart<TY, LANES, E, ODD>::load(u1, static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
@@ -275,9 +340,17 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward
       RowPart<TX, LANES, E, ODD>::load(u2, static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
       RowPart<TY, LANES, E, ODD>::load(q, static_cast<const TY*>(a.dh) + row * a.lddh, lane, a.width);
       const float mean = a.stats[2 * a.rows + row], r2 = a.stats[3 * a.rows + row];
+      float W2[E];
+      vector(2, W2);
+      if (a.y) {
+        float A[E], B[E];
+        vector(0, A);
+        vector(1, B);
+#pragma unroll
+        for (int e = 0; e < E; ++e) u2[e] = fmaf(act[e], fmaf(u1[e], A[e], B[e]), u2[e]);
+      }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (a.y) u2[e] = fmaf(act[e], fmaf(u1[e], A[e], B[e]), u2[e]);
         u2[e] = in_row<E, LANES>(e, lane, a.width) ? (u2[e] - mean) * r2 : 0.0f;
         P3[e] = fmaf(q[e], u2[e], P3[e]);
         P4[e] += q[e];
@@ -294,7 +367,9 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward
     if (a.dx) RowPart<TX, LANES, E, ODD>::store(d, static_cast<TX*>(a.dx) + row * a.lddx, lane, a.width);
     if (a.y) {
       float s[3] = {0.0f, 0.0f, 0.0f};
-      float dg[E];
+      float dg[E], A[E], B[E];
+      vector(0, A);
+      vector(1, B);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float t = d[e] * fmaf(u1[e], A[e], B[e]);
@@ -324,6 +399,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward
   }
   if (!a.partial) return;
   // column sums of the workgroup: its ROWS row groups in order, then one partial row per sum
+  float* cols = reinterpret_cast<float*>(store);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (!(a.partials >> k & 1)) continue;
@@ -336,12 +412,12 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward
     } else {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < E; ++e) cols[(threadIdx.x / LANES) * (LANES * E) + ((e >> 2) * LANES + lane) * 4 + (e & 3)] = P[e];
+      for (int e = 0; e < E; ++e) cols[(threadIdx.x / LANES) * W + ((e >> 2) * LANES + lane) * 4 + (e & 3)] = P[e];
       __syncthreads();
       for (int c = threadIdx.x; c < a.width; c += THREADS) {
         float s = 0.0f;
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) s += cols[r * (LANES * E) + c];
+        for (int r = 0; r < ROWS; ++r) s += cols[r * W + c];
         to[c] = s;
       }
     }
@@ -350,7 +426,7 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_backward
 
 template <typename TX, typename TY, bool BACK, int LANES, int E>
 int residual_launch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
-  constexpr int THREADS = LANES > 256 ? LANES : 256;
+  constexpr int THREADS = BACK ? residual_back_threads(LANES, E) : LANES > 256 ? LANES : 256;
   if (a.width % 4) {
     if (BACK) hipLaunchKernelGGL((k_residual_backward<TX, TY, LANES, E, true>), dim3(grid), dim3(THREADS), 0, stream, a);
     else hipLaunchKernelGGL((k_residual_forward<TX, TY, LANES, E, true>), dim3(grid), dim3(THREADS), 0, stream, a);

@@ -34,13 +34,25 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   __shared__ double part[4][64][16];
   const int cl = threadIdx.x & 15, slice = threadIdx.x >> 4;
   const int c = blockIdx.x * 16 + cl;
+  double s[4] = {0.0, 0.0, 0.0, 0.0};
+  if (c < a.width) {
+    // four groups of all sums in flight: each load waits for memory that another workgroup wrote
+    const float* p = a.partial + (int64_t)slice * 4 * a.width + c;
+    const int64_t step = 64 * 4 * (int64_t)a.width;
+    for (int64_t g = slice; g < a.groups; g += 64 * 4, p += 4 * step) {
+      float v[4][4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    double s = 0.0;
-    if (c < a.width && (a.partials >> k & 1))
-      for (int64_t g = slice; g < a.groups; g += 64) s += (double)a.partial[(g * 4 + k) * a.width + c];
-    part[k][slice][cl] = s;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[i][k] = (a.partials >> k & 1) && g + 64 * i < a.groups ? p[i * step + (int64_t)k * a.width] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[k] += (double)v[i][k];
+    }
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) part[k][slice][cl] = s[k];
   __syncthreads();
   for (int o = 32; o > 0; o >>= 1) {
     if (slice < o)
@@ -51,7 +63,7 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   if (slice != 0 || c >= a.width) return;
   const double P1 = part[0][0][cl], P2 = part[1][0][cl];
   const double w = a.w1 ? (double)param_at(a.w1, a.param_type, c) : 1.0, b = a.b1 ? (double)param_at(a.b1, a.param_type, c) : 0.0;
-  const double s = (double)a.scale * (a.lam ? (double)param_at(a.lam, a.param_type, c) : 1.0);
+  const double scale = (double)a.scale * (a.lam ? (double)param_at(a.lam, a.param_type, c) : 1.0);
   double gate = 1.0, slope = 0.0;
   if (a.channel) {
     const double g = (double)param_at(a.g, a.param_type, c);
@@ -59,11 +71,11 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
     else if (a.act == DISCO_ACT_TANH) { gate = tanh(g); slope = 1.0 - gate * gate; }
     else { gate = g; slope = 1.0; }
   }
-  if (a.dw1) param_put(a.dw1, a.param_type, c, s * gate * P1);
-  if (a.db1) param_put(a.db1, a.param_type, c, s * gate * P2);
+  if (a.dw1) param_put(a.dw1, a.param_type, c, scale * gate * P1);
+  if (a.db1) param_put(a.db1, a.param_type, c, scale * gate * P2);
   const double T = w * P1 + b * P2;
   if (a.dlam) param_put(a.dlam, a.param_type, c, (double)a.scale * gate * T);
-  if (a.channel && a.dg) param_put(a.dg, a.param_type, c, s * slope * T);
+  if (a.channel && a.dg) param_put(a.dg, a.param_type, c, scale * slope * T);
   if (a.dw2) param_put(a.dw2, a.param_type, c, part[2][0][cl]);
   if (a.db2) param_put(a.db2, a.param_type, c, part[3][0][cl]);
 }
@@ -99,13 +111,20 @@ static void fill(const disco_residual_norm* d, ResidualArgs* a) {
   a->w1 = d->post_weight; a->b1 = d->post_bias; a->w2 = d->pre_weight; a->b2 = d->pre_bias; a->lam = d->scale_vector;
 }
 
-static unsigned turns(int64_t rows, const ResidualShape& s, int64_t most) {
-  const int64_t at_a_time = s.threads / s.lanes, want = (rows + at_a_time - 1) / at_a_time;
+// Workgroups of a launch: about what the 256 compute units hold at once, each walks its share of the rows.
+static unsigned groups(int64_t rows, int threads, int lanes, int64_t most) {
+  const int64_t at_a_time = threads / lanes, want = (rows + at_a_time - 1) / at_a_time;
   return (unsigned)(want < most ? want : most);
 }
-// workgroups of a launch: every compute unit (256) can hold all of them at once, each walks its share of the rows
-static unsigned forward_grid(int64_t rows, const ResidualShape& s) { return turns(rows, s, 2048 * 256 / s.threads); }
-static unsigned backward_grid(int64_t rows, const ResidualShape& s) { return turns(rows, s, 1024 * 256 / s.threads); }
+static unsigned forward_grid(int64_t rows, const ResidualShape& s) {
+  const int threads = s.lanes > 256 ? s.lanes : 256;
+  return groups(rows, threads, s.lanes, 2048 * 256 / threads);
+}
+// The backward's number is also the number of partial sums that the finish reads again.
+static unsigned backward_grid(int64_t rows, const ResidualShape& s) {
+  const int threads = residual_back_threads(s.lanes, s.elems);
+  return groups(rows, threads, s.lanes, threads > 256 ? 256 : s.elems <= 8 ? 1024 : 512);
+}
 
 static bool strided(int64_t ld, int64_t rows, int64_t width) { return rows <= 1 || ld >= width; }
 
