@@ -17,6 +17,8 @@
 #ifndef DISCO_RESIDUAL_H
 #define DISCO_RESIDUAL_H
 
+#include <type_traits>
+
 #include "disco_internal.h"
 
 namespace disco {
@@ -37,17 +39,41 @@ struct ResidualArgs {
 
 enum ResidualPair { kPairF32 = 0, kPairF16 = 1, kPairBF16 = 2, kPairF32F16 = 3, kPairF32BF16 = 4 };
 
-// A kernel variant: lanes per row and elements a lane holds.
+// A kernel variant: lanes per row and elements a lane holds.  A row takes the first variant that holds it.  Blocks of 16
+// bits take eight elements a lane where float32 takes four, and half the lanes: the same bytes in flight for each wave
+// (HALVES).
 struct ResidualShape { int lanes, elems; };
-inline ResidualShape residual_shape(int64_t width) {
-  const int table[][2] = {{16, 4}, {32, 4}, {64, 4}, {64, 8}, {64, 12}, {64, 16}, {256, 8}, {256, 16}, {512, 16}, {1024, 16}};
-  for (const auto& t : table)
-    if (width <= (int64_t)t[0] * t[1]) return {t[0], t[1]};
+constexpr ResidualShape kResidualShapes[] = {{16, 4}, {32, 4}, {64, 4}, {64, 8}, {64, 12}, {64, 16}, {128, 12},
+                                             {256, 8}, {256, 12}, {256, 16}, {512, 12}, {512, 16}, {1024, 16}};
+constexpr ResidualShape residual_shape(int64_t width, bool halves) {
+  for (const ResidualShape& s : kResidualShapes)
+    if (width <= (int64_t)s.lanes * s.elems) return halves && s.elems == 4 ? ResidualShape{s.lanes / 2, 8} : s;
   return {0, 0};
 }
+// the smallest width of a variant: vectors inside it need no check
+constexpr int residual_least(int lanes, int elems) {
+  int least = 1;
+  for (const ResidualShape& s : kResidualShapes) {
+    if ((s.lanes == lanes && s.elems == elems) || (s.elems == 4 && s.lanes == 2 * lanes && elems == 8)) break;
+    least = s.lanes * s.elems + 1;
+  }
+  return least;
+}
 
-// lanes of a workgroup of the backward (see there)
-constexpr int residual_back_threads(int lanes, int elems) { return lanes > 64 ? lanes : elems <= 8 ? 1024 : elems <= 12 ? 768 : 512; }
+// lanes of a workgroup: four rows of a wave or more of less, or one row that takes several waves
+constexpr int residual_threads(int lanes) { return lanes > 64 ? lanes : 256; }
+// What a launch is for: the norm of x alone, the join, or the join with a gate for each element.  (One kernel for all three
+// would hold the registers of the last: the norm needs half of them.)
+enum ResidualMode { kNormOnly = 0, kJoin = 1, kJoinGated = 2 };
+inline int residual_mode(bool block, int gate) { return !block ? kNormOnly : gate == DISCO_GATE_FULL ? kJoinGated : kJoin; }
+// ... of the backward (see there): waves of a SIMD, by their registers; the norm alone has room for more and is faster with
+// these (half rows of 1433: 272 us with two, 310 with three and four; float32 rows of 1000: 236 with two, 255 with four)
+constexpr int residual_back_waves(int lanes, int elems, int mode) {
+  return lanes == 1024 || elems <= 4 ? 4
+         : mode == kNormOnly ? (elems <= 8 ? 4 : elems > 12 || lanes == 128 ? 2 : lanes == 512 ? 4 : 3)
+         : lanes == 512 || elems > 12 ? 2 : elems <= 8 ? 4 - (mode == kJoinGated) : 3 - (lanes == 256 || mode == kJoinGated);
+}
+constexpr int residual_back_threads(int lanes, int elems, int mode) { return lanes > 64 ? lanes : 256 * residual_back_waves(lanes, elems, mode); }
 
 // grid: workgroups; a workgroup takes rows / (its rows at a time * grid) turns
 template <int PAIR> int residual_forward(const ResidualArgs& a, unsigned grid, hipStream_t stream);
@@ -55,13 +81,9 @@ template <int PAIR> int residual_backward(const ResidualArgs& a, unsigned grid, 
 
 #if defined(DISCO_RESIDUAL_KERNELS)
 
-template <int T> struct TypeOf;
-template <> struct TypeOf<DISCO_F32> { typedef float type; };
-template <> struct TypeOf<DISCO_F16> { typedef _Float16 type; };
-template <> struct TypeOf<DISCO_BF16> { typedef __bf16 type; };
-
 __device__ __forceinline__ float activate(float g, int act) {
-  if (act == DISCO_ACT_SIGMOID) return 1.0f / (1.0f + expf(-g));
+  // the reciprocal instruction (1 ulp) rather than a division: a gate for each element is arithmetic that shows
+  if (act == DISCO_ACT_SIGMOID) return __builtin_amdgcn_rcpf(1.0f + expf(-g));
   if (act == DISCO_ACT_TANH) return tanhf(g);
   return g;
 }
@@ -77,22 +99,56 @@ __device__ __forceinline__ float activate_slope(float a, int act) {
 // four, so the row's last vector is partial.
 template <typename T, int LANES, int E, bool ODD>
 struct RowPart {
+  static constexpr int LEAST = residual_least(LANES, E);
   typedef T vec __attribute__((ext_vector_type(4), aligned(sizeof(T))));
-  __device__ static __forceinline__ void load(float (&r)[E], const T* p, int lane, int width) {
+  // No branch around a load, so that all of a row's are in flight together (behind branches half rows of 1434 moved
+  // 2.9 TB/s, of 1436 4.1): a vector that reaches behind the row is read from the row's end instead and shifted down;
+  // elements behind the width are zero.
+  struct Raw { vec v[E / 4]; };
+  __device__ static __forceinline__ Raw fetch(const T* p, int lane, int width) {
+    Raw r;
+    if (LEAST == 1 && ODD && width < 4) {
+      const int c = lane * 4;
+#pragma unroll
+      for (int k = 0; k < E / 4; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) r.v[k][e] = k == 0 && c + e < width ? p[c + e] : (T)0.0f;
+      return r;
+    }
 #pragma unroll
     for (int k = 0; k < E / 4; ++k) {
       const int c = (k * LANES + lane) * 4;
-      vec v = {};
-      if (c + 4 <= width) {
-        v = *reinterpret_cast<const vec*>(p + c);
-      } else if (ODD && c < width) {
-        v.x = p[c];
-        if (c + 1 < width) v.y = p[c + 1];
-        if (c + 2 < width) v.z = p[c + 2];
+      r.v[k] = *reinterpret_cast<const vec*>(p + ((k + 1) * LANES * 4 <= LEAST ? c : min(c, width - 4)));
+    }
+    return r;
+  }
+  __device__ static __forceinline__ void expand(const Raw& raw, float (&r)[E], int lane, int width) {
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k) {
+      float t[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = (float)raw.v[k][e];
+      if ((k + 1) * LANES * 4 > LEAST && !(LEAST == 1 && ODD && width < 4)) {
+        const int over = (k * LANES + lane) * 4 + 4 - width;      // elements of this vector behind the row, if positive
+        if (ODD) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float u = over <= 0 ? t[e] : 0.0f;
+            if (e < 3) u = over == 1 ? t[e < 3 ? e + 1 : 3] : u;
+            if (e < 2) u = over == 2 ? t[e < 2 ? e + 2 : 3] : u;
+            if (e < 1) u = over == 3 ? t[3] : u;
+            t[e] = u;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = over <= 0 ? t[e] : 0.0f;
+        }
       }
-      r[4 * k] = (float)v.x; r[4 * k + 1] = (float)v.y; r[4 * k + 2] = (float)v.z; r[4 * k + 3] = (float)v.w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[4 * k + e] = t[e];
     }
   }
+  __device__ static __forceinline__ void load(float (&r)[E], const T* p, int lane, int width) { expand(fetch(p, lane, width), r, lane, width); }
   __device__ static __forceinline__ void store(const float (&r)[E], T* p, int lane, int width) {
 #pragma unroll
     for (int k = 0; k < E / 4; ++k) {
@@ -135,8 +191,9 @@ __device__ __forceinline__ void row_sum(float (&v)[R], float4* lds, int& turn) {
   for (int r = 0; r < R; ++r) v[r] = add_dpp<0x4E>(v[r]);       // quad_perm [2, 3, 0, 1]
 #pragma unroll
   for (int r = 0; r < R; ++r) v[r] = add_dpp<0x141>(v[r]);      // row_half_mirror
+  if constexpr (LANES >= 16)
 #pragma unroll
-  for (int r = 0; r < R; ++r) v[r] = add_dpp<0x140>(v[r]);      // row_mirror
+    for (int r = 0; r < R; ++r) v[r] = add_dpp<0x140>(v[r]);    // row_mirror
   if constexpr (LANES >= 32)
 #pragma unroll
     for (int r = 0; r < R; ++r) v[r] = add_swap16(v[r]);
@@ -221,46 +278,57 @@ __device__ __forceinline__ void load_branch(const ResidualArgs& a, int lane, flo
   }
 }
 
-template <typename TX, typename TY, int LANES, int E, bool ODD>
-__global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_forward(const ResidualArgs a) {
-  constexpr int THREADS = LANES > 256 ? LANES : 256, ROWS = THREADS / LANES;
+template <typename TX, typename TY, int MODE, int LANES, int E, bool ODD>
+__global__ __launch_bounds__(residual_threads(LANES)) void k_residual_forward(const ResidualArgs a) {
+  constexpr int THREADS = residual_threads(LANES), ROWS = THREADS / LANES;
+  constexpr bool BLOCK = MODE != kNormOnly, FULL = MODE == kJoinGated;
+  typedef RowPart<TX, LANES, E, ODD> PX;
+  typedef RowPart<TY, LANES, E, ODD> PY;
   __shared__ float4 lds[LANES > 64 ? 2 * (LANES / 64) : 1];
   const int lane = threadIdx.x % LANES;
   int turn = 0;
   float A[E], B[E], W2[E], B2[E];
-  if (a.y) load_branch<LANES, E, ODD>(a, lane, A, B);
-  if (a.pre) {
+  if constexpr (BLOCK) load_branch<LANES, E, ODD>(a, lane, A, B);
+  if (!BLOCK || a.pre) {
     load_vector<LANES, E, ODD>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
     load_vector<LANES, E, ODD>(a.b2, a.param_type, lane, a.width, 0.0f, B2);
   }
   for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
-    float o[E];
-    RowPart<TX, LANES, E, ODD>::load(o, static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
-    if (a.y) {
-      float z[E], g[E], grow = 1.0f, mean, rstd;
-      RowPart<TY, LANES, E, ODD>::load(z, static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
-      if (a.gate == DISCO_GATE_FULL) RowPart<TY, LANES, E, ODD>::load(g, static_cast<const TY*>(a.g) + row * a.ldg, lane, a.width);
-      if (a.gate == DISCO_GATE_ROW) grow = activate((float)static_cast<const TY*>(a.g)[row * a.ldg], a.act);
+    // all of the row's loads, before any of them is waited for
+    typename PY::Raw ry, rg;
+    float o[E], z[E], g[E], grow = 1.0f;
+    const typename PX::Raw rx = PX::fetch(static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
+    if constexpr (BLOCK) {
+      ry = PY::fetch(static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
+      if constexpr (FULL) rg = PY::fetch(static_cast<const TY*>(a.g) + row * a.ldg, lane, a.width);
+      else if (a.gate == DISCO_GATE_ROW) grow = (float)static_cast<const TY*>(a.g)[row * a.ldg];
+    }
+    PX::expand(rx, o, lane, a.width);
+    if constexpr (BLOCK) {
+      PY::expand(ry, z, lane, a.width);
+      if constexpr (FULL) PY::expand(rg, g, lane, a.width);
+      if (!FULL && a.gate == DISCO_GATE_ROW) grow = activate(grow, a.act);
       if (a.post) {
+        float mean, rstd;
         standardise<LANES, E>(z, a.post, a.eps, a.inv_width, lane, a.width, lds, turn, mean, rstd);
         if (a.stats && lane == 0) { a.stats[row] = mean; a.stats[a.rows + row] = rstd; }
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         float t = fmaf(z[e], A[e], B[e]);
-        if (a.gate == DISCO_GATE_FULL) t *= activate(g[e], a.act);
-        if (a.gate == DISCO_GATE_ROW) t *= grow;
+        if constexpr (FULL) t *= activate(g[e], a.act);
+        else t *= grow;
         o[e] += t;
       }
-      RowPart<TX, LANES, E, ODD>::store(o, static_cast<TX*>(a.out) + row * a.ldo, lane, a.width);
+      PX::store(o, static_cast<TX*>(a.out) + row * a.ldo, lane, a.width);
     }
-    if (a.pre) {
+    if (!BLOCK || a.pre) {
       float mean, rstd;
       standardise<LANES, E>(o, a.pre, a.eps, a.inv_width, lane, a.width, lds, turn, mean, rstd);
       if (a.stats && lane == 0) { a.stats[2 * a.rows + row] = mean; a.stats[3 * a.rows + row] = rstd; }
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], W2[e], B2[e]);
-      RowPart<TY, LANES, E, ODD>::store(o, static_cast<TY*>(a.h) + row * a.ldh, lane, a.width);
+      PY::store(o, static_cast<TY*>(a.h) + row * a.ldh, lane, a.width);
     }
   }
 }
@@ -269,34 +337,42 @@ __global__ __launch_bounds__(LANES > 256 ? LANES : 256) void k_residual_forward(
 // vectors that every row needs again stay in LDS (12 bytes an element beside the 20 to 32 that the row moves through memory):
 // in registers they cost a third of the waves that a compute unit can hold.  Rows of a wave or less share a workgroup as
 // large as the registers allow, since each workgroup leaves one partial row per sum behind for the finish to read.
-template <typename TX, typename TY, int LANES, int E, bool ODD>
-__global__ __launch_bounds__(residual_back_threads(LANES, E), LANES < 1024 && E > 12 ? 2 : LANES == 256 ? 4 : 1) void k_residual_backward(const ResidualArgs a) {
-  constexpr int THREADS = residual_back_threads(LANES, E), ROWS = THREADS / LANES, W = LANES * E;
+template <typename TX, typename TY, int MODE, int LANES, int E, bool ODD>
+__global__ __launch_bounds__(residual_back_threads(LANES, E, MODE), residual_back_waves(LANES, E, MODE)) void k_residual_backward(const ResidualArgs a) {
+  constexpr bool BLOCK = MODE != kNormOnly, FULL = MODE == kJoinGated;
+  constexpr int THREADS = residual_back_threads(LANES, E, MODE), ROWS = THREADS / LANES, W = LANES * E;
   __shared__ float4 lds[LANES > 64 ? 2 * (LANES / 64) : 1];
   // the vectors; after the last row, for rows of a wave or less, the column sums of the workgroup's row groups
   __shared__ float4 store[(W <= 8192 ? (ROWS > 3 ? ROWS : 3) * W : 4) / 4];
-  constexpr bool IN_LDS = W <= 8192;
+  constexpr bool IN_LDS = W <= 8192, AHEAD = LANES == 512 && MODE == kJoin && (E == 12 || sizeof(TX) == 2);
+  typedef RowPart<TX, LANES, E, ODD> PX;
+  typedef RowPart<TY, LANES, E, ODD> PY;
   const int lane = threadIdx.x % LANES;
   int turn = 0;
   float regs[IN_LDS ? 1 : 3][E], P1[E], P2[E], P3[E], P4[E];
   {
     float A[E], B[E], W2[E];
     if (!IN_LDS || threadIdx.x < LANES) {
-      load_branch<LANES, E, ODD>(a, lane, A, B);
+      if constexpr (BLOCK) load_branch<LANES, E, ODD>(a, lane, A, B);
       load_vector<LANES, E, ODD>(a.w2, a.param_type, lane, a.width, 1.0f, W2);
     }
     if constexpr (IN_LDS) {
       if (threadIdx.x < LANES)
 #pragma unroll
         for (int k = 0; k < E / 4; ++k) {
-          store[k * LANES + lane] = make_float4(A[4 * k], A[4 * k + 1], A[4 * k + 2], A[4 * k + 3]);
-          store[W / 4 + k * LANES + lane] = make_float4(B[4 * k], B[4 * k + 1], B[4 * k + 2], B[4 * k + 3]);
+          if constexpr (BLOCK) {
+            store[k * LANES + lane] = make_float4(A[4 * k], A[4 * k + 1], A[4 * k + 2], A[4 * k + 3]);
+            store[W / 4 + k * LANES + lane] = make_float4(B[4 * k], B[4 * k + 1], B[4 * k + 2], B[4 * k + 3]);
+          }
           store[W / 2 + k * LANES + lane] = make_float4(W2[4 * k], W2[4 * k + 1], W2[4 * k + 2], W2[4 * k + 3]);
         }
       __syncthreads();
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e) { regs[0][e] = A[e]; regs[1][e] = B[e]; regs[2][e] = W2[e]; }
+      for (int e = 0; e < E; ++e) {
+        if constexpr (BLOCK) { regs[0][e] = A[e]; regs[1][e] = B[e]; }
+        regs[2][e] = W2[e];
+      }
     }
   }
   const auto vector = [&](int which, float (&v)[E]) {
@@ -313,45 +389,82 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E), LANES < 1024 && E 
   };
 #pragma unroll
   for (int e = 0; e < E; ++e) P1[e] = P2[e] = P3[e] = P4[e] = 0.0f;
-  for (int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
-    if constexpr (IN_LDS) asm volatile("" ::: "memory");      // the vectors are read again, not kept in registers
-    float u1[E], act[E], d[E], r1 = 1.0f, grow = 1.0f;
-    if (a.y) {
-      RowPart<TY, LANES, E, ODD>::load(u1, static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
-      if (a.gate == DISCO_GATE_FULL) RowPart<TY, LANES, E, ODD>::load(act, static_cast<const TY*>(a.g) + row * a.ldg, lane, a.width);
-      if (a.gate == DISCO_GATE_ROW) grow = activate((float)static_cast<const TY*>(a.g)[row * a.ldg], a.act);
+  typename PX::Raw rx, rdo;
+  typename PY::Raw ry, rg, rdh;
+  float m1 = 0.0f, r1 = 1.0f, m2 = 0.0f, r2 = 1.0f, grow = 1.0f;
+  // A row's loads, all before any of them is waited for; with a gate for each element in two parts, which takes fewer
+  // registers (169343 x 256: 267 us, 281 in one).  AHEAD: the next row's are under way during this one's work -- for rows of
+  // eight waves, of which a compute unit holds one (half rows of 5000: 547 us, 643 without).
+  const auto fetch = [&](int64_t row) {
+    if constexpr (BLOCK) {
+      ry = PY::fetch(static_cast<const TY*>(a.y) + row * a.ldy, lane, a.width);
+      if constexpr (FULL) rg = PY::fetch(static_cast<const TY*>(a.g) + row * a.ldg, lane, a.width);
+      else if (a.gate == DISCO_GATE_ROW) grow = (float)static_cast<const TY*>(a.g)[row * a.ldg];
       if (a.post) {
-        const float mean = a.stats[row];
+        m1 = a.stats[row];
         r1 = a.stats[a.rows + row];
-#pragma unroll
-        for (int e = 0; e < E; ++e) u1[e] = in_row<E, LANES>(e, lane, a.width) ? (u1[e] - mean) * r1 : 0.0f;
       }
-#pragma unroll
-      for (int e = 0; e < E; ++e) act[e] = a.gate == DISCO_GATE_FULL ? activate(act[e], a.act) : grow;
     }
-    if (a.dout) {
-      RowPart<TX, LANES, E, ODD>::load(d, static_cast<const TX*>(a.dout) + row * a.lddo, lane, a.width);
+  };
+  const auto fetch_sum = [&](int64_t row) {
+    if (!BLOCK || a.dh) {
+      rx = PX::fetch(static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
+      rdh = PY::fetch(static_cast<const TY*>(a.dh) + row * a.lddh, lane, a.width);
+      m2 = a.stats[2 * a.rows + row];
+      r2 = a.stats[3 * a.rows + row];
+    }
+    if (BLOCK && a.dout) rdo = PX::fetch(static_cast<const TX*>(a.dout) + row * a.lddo, lane, a.width);
+  };
+  int64_t row = (int64_t)blockIdx.x * ROWS + threadIdx.x / LANES;
+  if (AHEAD && row < a.rows) { fetch(row); fetch_sum(row); }
+  while (row < a.rows) {
+    if constexpr (IN_LDS) asm volatile("" ::: "memory");      // the vectors are read again, not kept in registers
+    const int64_t next = row + (int64_t)gridDim.x * ROWS;
+    if (!AHEAD) { fetch(row); if (!FULL) fetch_sum(row); }
+    const typename PY::Raw cy = ry, cg = rg;
+    const float mean1 = m1, rstd1 = r1;
+    typename PX::Raw cx = rx, cdo = rdo;
+    typename PY::Raw cdh = rdh;
+    float mean2 = m2, rstd2 = r2;
+    float u1[E], act[FULL ? E : 1], d[E], gate = grow;
+    if (AHEAD && next < a.rows) { fetch(next); fetch_sum(next); }
+    if constexpr (BLOCK) {
+      PY::expand(cy, u1, lane, a.width);
+      if (a.post)
+#pragma unroll
+        for (int e = 0; e < E; ++e) u1[e] = in_row<E, LANES>(e, lane, a.width) ? (u1[e] - mean1) * rstd1 : 0.0f;
+      if constexpr (FULL) {
+        PY::expand(cg, act, lane, a.width);
+#pragma unroll
+        for (int e = 0; e < E; ++e) act[e] = activate(act[e], a.act);
+      } else {
+        if (a.gate == DISCO_GATE_ROW) gate = activate(gate, a.act);
+        act[0] = gate;
+      }
+    }
+    if (FULL) { fetch_sum(row); cx = rx; cdo = rdo; cdh = rdh; mean2 = m2; rstd2 = r2; }
+    const auto gated = [&](int e) { return act[FULL ? e : 0]; };
+    if (BLOCK && a.dout) {
+      PX::expand(cdo, d, lane, a.width);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) d[e] = 0.0f;
     }
-    if (a.dh) {
-      float u2[E], q[E], s[2] = {0.0f, 0.0f};
-      RowPart<TX, LANES, E, ODD>::load(u2, static_cast<const TX*>(a.x) + row * a.ldx, lane, a.width);
-      RowPart<TY, LANES, E, ODD>::load(q, static_cast<const TY*>(a.dh) + row * a.lddh, lane, a.width);
-      const float mean = a.stats[2 * a.rows + row], r2 = a.stats[3 * a.rows + row];
-      float W2[E];
+    if (!BLOCK || a.dh) {
+      float s[2] = {0.0f, 0.0f}, W2[E], u2[E], q[E];
+      PX::expand(cx, u2, lane, a.width);
+      PY::expand(cdh, q, lane, a.width);
       vector(2, W2);
-      if (a.y) {
+      if constexpr (BLOCK) {
         float A[E], B[E];
         vector(0, A);
         vector(1, B);
 #pragma unroll
-        for (int e = 0; e < E; ++e) u2[e] = fmaf(act[e], fmaf(u1[e], A[e], B[e]), u2[e]);
+        for (int e = 0; e < E; ++e) u2[e] = fmaf(gated(e), fmaf(u1[e], A[e], B[e]), u2[e]);
       }
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        u2[e] = in_row<E, LANES>(e, lane, a.width) ? (u2[e] - mean) * r2 : 0.0f;
+        u2[e] = in_row<E, LANES>(e, lane, a.width) ? (u2[e] - mean2) * rstd2 : 0.0f;
         P3[e] = fmaf(q[e], u2[e], P3[e]);
         P4[e] += q[e];
         q[e] *= W2[e];
@@ -362,40 +475,41 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E), LANES < 1024 && E 
       const float mq = a.pre == DISCO_NORM_LAYER ? s[1] * a.inv_width : 0.0f, mqu = s[0] * a.inv_width;
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        d[e] += in_row<E, LANES>(e, lane, a.width) ? r2 * (q[e] - mq - u2[e] * mqu) : 0.0f;
+        d[e] += in_row<E, LANES>(e, lane, a.width) ? rstd2 * (q[e] - mq - u2[e] * mqu) : 0.0f;
     }
-    if (a.dx) RowPart<TX, LANES, E, ODD>::store(d, static_cast<TX*>(a.dx) + row * a.lddx, lane, a.width);
-    if (a.y) {
+    if (a.dx) PX::store(d, static_cast<TX*>(a.dx) + row * a.lddx, lane, a.width);
+    if constexpr (BLOCK) {
       float s[3] = {0.0f, 0.0f, 0.0f};
-      float dg[E], A[E], B[E];
+      float dg[FULL ? E : 1], A[E], B[E];
       vector(0, A);
       vector(1, B);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float t = d[e] * fmaf(u1[e], A[e], B[e]);
         s[2] += t;
-        dg[e] = t * activate_slope(act[e], a.act);
-        d[e] *= act[e];
+        if constexpr (FULL) dg[e] = t * activate_slope(act[e], a.act);
+        d[e] *= gated(e);
         P1[e] = fmaf(d[e], u1[e], P1[e]);
         P2[e] += d[e];
         d[e] *= A[e];
         s[0] = fmaf(d[e], u1[e], s[0]);
         s[1] += d[e];
       }
-      if (a.dg && a.gate == DISCO_GATE_FULL)
-        RowPart<TY, LANES, E, ODD>::store(dg, static_cast<TY*>(a.dg) + row * a.lddg, lane, a.width);
-      if (a.post || (a.dg && a.gate == DISCO_GATE_ROW)) row_sum<LANES, 3>(s, lds, turn);
-      if (a.dg && a.gate == DISCO_GATE_ROW && lane == 0)
-        static_cast<TY*>(a.dg)[row * a.lddg] = (TY)(s[2] * activate_slope(grow, a.act));
+      if constexpr (FULL)
+        if (a.dg) PY::store(dg, static_cast<TY*>(a.dg) + row * a.lddg, lane, a.width);
+      if (a.post || (!FULL && a.dg)) row_sum<LANES, 3>(s, lds, turn);
+      if (!FULL && a.dg && lane == 0)
+        static_cast<TY*>(a.dg)[row * a.lddg] = (TY)(s[2] * activate_slope(gate, a.act));
       if (a.dy) {
         if (a.post) {
           const float mp = a.post == DISCO_NORM_LAYER ? s[1] * a.inv_width : 0.0f, mpu = s[0] * a.inv_width;
 #pragma unroll
-          for (int e = 0; e < E; ++e) d[e] = r1 * (d[e] - mp - u1[e] * mpu);
+          for (int e = 0; e < E; ++e) d[e] = rstd1 * (d[e] - mp - u1[e] * mpu);
         }
-        RowPart<TY, LANES, E, ODD>::store(d, static_cast<TY*>(a.dy) + row * a.lddy, lane, a.width);
+        PY::store(d, static_cast<TY*>(a.dy) + row * a.lddy, lane, a.width);
       }
     }
+    row = next;
   }
   if (!a.partial) return;
   // column sums of the workgroup: its ROWS row groups in order, then one partial row per sum
@@ -426,30 +540,42 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E), LANES < 1024 && E 
 
 template <typename TX, typename TY, bool BACK, int LANES, int E>
 int residual_launch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
-  constexpr int THREADS = BACK ? residual_back_threads(LANES, E) : LANES > 256 ? LANES : 256;
-  if (a.width % 4) {
-    if (BACK) hipLaunchKernelGGL((k_residual_backward<TX, TY, LANES, E, true>), dim3(grid), dim3(THREADS), 0, stream, a);
-    else hipLaunchKernelGGL((k_residual_forward<TX, TY, LANES, E, true>), dim3(grid), dim3(THREADS), 0, stream, a);
-  } else {
-    if (BACK) hipLaunchKernelGGL((k_residual_backward<TX, TY, LANES, E, false>), dim3(grid), dim3(THREADS), 0, stream, a);
-    else hipLaunchKernelGGL((k_residual_forward<TX, TY, LANES, E, false>), dim3(grid), dim3(THREADS), 0, stream, a);
-  }
+  const int mode = residual_mode(a.y != nullptr, a.gate);
+  const dim3 threads(BACK ? residual_back_threads(LANES, E, mode) : residual_threads(LANES));
+  auto launch = [&](auto which, auto odd) {
+    constexpr int M = decltype(which)::value;
+    constexpr bool O = decltype(odd)::value;
+    if constexpr (BACK) hipLaunchKernelGGL((k_residual_backward<TX, TY, M, LANES, E, O>), dim3(grid), threads, 0, stream, a);
+    else hipLaunchKernelGGL((k_residual_forward<TX, TY, M, LANES, E, O>), dim3(grid), threads, 0, stream, a);
+  };
+  auto by_mode = [&](auto odd) {
+    if (mode == kNormOnly) launch(std::integral_constant<int, kNormOnly>(), odd);
+    else if (mode == kJoin) launch(std::integral_constant<int, kJoin>(), odd);
+    else launch(std::integral_constant<int, kJoinGated>(), odd);
+  };
+  if (a.width % 4) by_mode(std::true_type());
+  else by_mode(std::false_type());
   DISCO_CHECK_LAUNCH();
   return DISCO_OK;
 }
 
 template <typename TX, typename TY, bool BACK>
 int residual_dispatch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
-  const ResidualShape s = residual_shape(a.width);
+  constexpr bool HALVES = sizeof(TY) == 2;
+  constexpr int N = HALVES ? 2 : 1;      // the three narrowest variants
+  const ResidualShape s = residual_shape(a.width, HALVES);
   switch (s.lanes * 100 + s.elems) {
-    case 1604: return residual_launch<TX, TY, BACK, 16, 4>(a, grid, stream);
-    case 3204: return residual_launch<TX, TY, BACK, 32, 4>(a, grid, stream);
-    case 6404: return residual_launch<TX, TY, BACK, 64, 4>(a, grid, stream);
+    case 1600 / N + 4 * N: return residual_launch<TX, TY, BACK, 16 / N, 4 * N>(a, grid, stream);
+    case 3200 / N + 4 * N: return residual_launch<TX, TY, BACK, 32 / N, 4 * N>(a, grid, stream);
+    case 6400 / N + 4 * N: return residual_launch<TX, TY, BACK, 64 / N, 4 * N>(a, grid, stream);
     case 6408: return residual_launch<TX, TY, BACK, 64, 8>(a, grid, stream);
     case 6412: return residual_launch<TX, TY, BACK, 64, 12>(a, grid, stream);
     case 6416: return residual_launch<TX, TY, BACK, 64, 16>(a, grid, stream);
+    case 12812: return residual_launch<TX, TY, BACK, 128, 12>(a, grid, stream);
     case 25608: return residual_launch<TX, TY, BACK, 256, 8>(a, grid, stream);
+    case 25612: return residual_launch<TX, TY, BACK, 256, 12>(a, grid, stream);
     case 25616: return residual_launch<TX, TY, BACK, 256, 16>(a, grid, stream);
+    case 51212: return residual_launch<TX, TY, BACK, 512, 12>(a, grid, stream);
     case 51216: return residual_launch<TX, TY, BACK, 512, 16>(a, grid, stream);
     case 102416: return residual_launch<TX, TY, BACK, 1024, 16>(a, grid, stream);
   }

@@ -3,6 +3,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "disco_residual.h"
 
 namespace disco {
@@ -34,6 +36,13 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   __shared__ double part[4][64][16];
   const int cl = threadIdx.x & 15, slice = threadIdx.x >> 4;
   const int c = blockIdx.x * 16 + cl;
+  double w = 1.0, b = 0.0, scale = (double)a.scale, g = 0.0;      // read while the sums come in
+  if (slice == 0 && c < a.width) {
+    if (a.w1) w = (double)param_at(a.w1, a.param_type, c);
+    if (a.b1) b = (double)param_at(a.b1, a.param_type, c);
+    if (a.lam) scale *= (double)param_at(a.lam, a.param_type, c);
+    if (a.channel) g = (double)param_at(a.g, a.param_type, c);
+  }
   double s[4] = {0.0, 0.0, 0.0, 0.0};
   if (c < a.width) {
     // four groups of all sums in flight: each load waits for memory that another workgroup wrote
@@ -62,11 +71,8 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   }
   if (slice != 0 || c >= a.width) return;
   const double P1 = part[0][0][cl], P2 = part[1][0][cl];
-  const double w = a.w1 ? (double)param_at(a.w1, a.param_type, c) : 1.0, b = a.b1 ? (double)param_at(a.b1, a.param_type, c) : 0.0;
-  const double scale = (double)a.scale * (a.lam ? (double)param_at(a.lam, a.param_type, c) : 1.0);
   double gate = 1.0, slope = 0.0;
   if (a.channel) {
-    const double g = (double)param_at(a.g, a.param_type, c);
     if (a.act == DISCO_ACT_SIGMOID) { gate = 1.0 / (1.0 + exp(-g)); slope = gate * (1.0 - gate); }
     else if (a.act == DISCO_ACT_TANH) { gate = tanh(g); slope = 1.0 - gate * gate; }
     else { gate = g; slope = 1.0; }
@@ -116,14 +122,23 @@ static unsigned groups(int64_t rows, int threads, int lanes, int64_t most) {
   const int64_t at_a_time = threads / lanes, want = (rows + at_a_time - 1) / at_a_time;
   return (unsigned)(want < most ? want : most);
 }
-static unsigned forward_grid(int64_t rows, const ResidualShape& s) {
-  const int threads = s.lanes > 256 ? s.lanes : 256;
-  return groups(rows, threads, s.lanes, 2048 * 256 / threads);
+// The forward's waves: as many as keep FETCHED bytes of rows on their way to a compute unit (HBM answers after about a
+// microsecond at 20 GB/s for each), and no more: each further wave is one more place that memory is read and written at.
+// Joins of 200 M values, float32 rows of 256: 287 us with 8 waves, 308 with 16, 343 with 32; half rows of 256: 297, 322, 351;
+// norms, with half the bytes a wave, need 16: 179 us with 8, 141 with 16, 150 with 32.  Rows that several waves share
+// wait for each other, and want more (half rows of 5000: 383 us with 8, 304 with 16); so do gates for each element, whose
+// arithmetic shows (169343 x 256: 180 us with 8, 157 with 12).
+static unsigned forward_grid(int64_t rows, const ResidualShape& s, int mode, bool wide_stream, bool halves) {
+  const int threads = residual_threads(s.lanes), y = halves ? 2 : 4, x = wide_stream ? 4 : 2;
+  const int bytes = 64 * s.elems * (x + (mode == kNormOnly ? 0 : mode == kJoin ? y : 2 * y));
+    const int fetched = (mode == kJoinGated ? 2 : 1) * (s.lanes <= 64 ? 16384 : s.lanes <= 256 ? 24576 : 32768);
+  const int waves = std::max(8, std::min(32, (fetched + bytes - 1) / bytes));
+  return groups(rows, threads, s.lanes, 256 * std::max(1, (waves * 64 + threads - 1) / threads));
 }
 // The backward's number is also the number of partial sums that the finish reads again.
-static unsigned backward_grid(int64_t rows, const ResidualShape& s) {
-  const int threads = residual_back_threads(s.lanes, s.elems);
-  return groups(rows, threads, s.lanes, threads > 256 ? 256 : s.elems <= 8 ? 1024 : 512);
+static unsigned backward_grid(int64_t rows, const ResidualShape& s, int mode) {
+  const int threads = residual_back_threads(s.lanes, s.elems, mode);
+  return groups(rows, threads, s.lanes, (int64_t)residual_back_waves(s.lanes, s.elems, mode) * 256 * 256 / threads);
 }
 
 static bool strided(int64_t ld, int64_t rows, int64_t width) { return rows <= 1 || ld >= width; }
@@ -145,8 +160,8 @@ extern "C" int disco_residual_norm_forward(const disco_residual_norm* d, void* o
   ResidualArgs a;
   fill(d, &a);
   a.out = out; a.ldo = ld_out; a.h = h; a.ldh = ld_h; a.stats = stats;
-  const ResidualShape s = residual_shape(F);
-  const unsigned grid = forward_grid(n, s);
+  const ResidualShape s = residual_shape(F, d->block_type != DISCO_F32);
+  const unsigned grid = forward_grid(n, s, residual_mode(d->has_block, d->gate_kind), d->stream_type == DISCO_F32, d->block_type != DISCO_F32);
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   switch (pair_of(d->stream_type, d->block_type)) {
     case kPairF32: return residual_forward<kPairF32>(a, grid, stream);
@@ -159,7 +174,10 @@ extern "C" int disco_residual_norm_forward(const disco_residual_norm* d, void* o
 
 extern "C" size_t disco_residual_norm_workspace_bytes(int64_t rows, int64_t width) {
   if (rows < 0 || width < 1 || width > DISCO_RESIDUAL_MAX_WIDTH) return 0;
-  return (size_t)backward_grid(rows, residual_shape(width)) * 4 * (size_t)width * sizeof(float);
+  unsigned most = 0;      // of any type and gate
+  for (const bool halves : {false, true})
+    for (const int mode : {kNormOnly, kJoin, kJoinGated}) most = std::max(most, backward_grid(rows, residual_shape(width, halves), mode));
+  return (size_t)most * 4 * (size_t)width * sizeof(float);
 }
 
 extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const float* stats, const disco_residual_norm_grads* g,
@@ -185,8 +203,8 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
     if (d->ldx < 0 || d->ldy < 0 || d->ld_gate < 0 || g->ld_dout < 0 || g->ld_dh < 0) return DISCO_EINVAL;
     if ((d->has_block && !d->y) || (g->dh && !d->x) || (d->gate_kind && !d->gate) || ((d->post_norm || g->dh) && !stats)) return DISCO_EINVAL;
   }
-  const ResidualShape s = residual_shape(F);
-  const unsigned grid = backward_grid(n, s);
+  const ResidualShape s = residual_shape(F, d->block_type != DISCO_F32);
+  const unsigned grid = backward_grid(n, s, residual_mode(d->has_block, d->gate_kind));
   const size_t need = (size_t)grid * 4 * (size_t)F * sizeof(float);
   if (a.partials && n > 0 && (!workspace || workspace_bytes < need)) return DISCO_EWORKSPACE;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
