@@ -6,8 +6,8 @@ nothing synchronises.  No counterpart in the reference, whose training loops do 
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+from array import array
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -15,22 +15,26 @@ import torch
 from . import _lib
 
 _NORMS = {1.0: 1, 2.0: 2, math.inf: 0}
+_SHARED = "clip_grads: two tensors share memory; each gradient may be scaled only once"
 
 
 def _tensors(grads) -> List[torch.Tensor]:
+    """The list of gradients.  The checks go list by list rather than tensor by tensor: a model has hundreds of them."""
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    for g in grads:
-        if not isinstance(g, torch.Tensor) or g.layout != torch.strided:
-            raise TypeError("gradients must be dense tensors")
-        if g.dtype not in _lib.DTYPES:
-            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
-        if g.device != grads[0].device:
-            raise ValueError(f"gradients on {grads[0].device} and {g.device}: one device at a time")
+    if not grads:
+        return grads
+    if not all([isinstance(g, torch.Tensor) and g.layout is torch.strided for g in grads]):
+        raise TypeError("gradients must be dense tensors")
+    if not {g.dtype for g in grads} <= _lib.DTYPES.keys():
+        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {sorted({str(g.dtype) for g in grads})}")
+    device = grads[0].device
+    if any([g.device != device for g in grads]):
+        raise ValueError(f"gradients on {sorted({str(g.device) for g in grads})}: one device at a time")
     return grads
 
 
 def _on_gpu(grads) -> None:
-    if grads and grads[0].device.type != "cuda":
+    if grads and not grads[0].is_cuda:
         raise RuntimeError(f"gradients on {grads[0].device}: disco_amd runs on the GPU only, there is no CPU fallback")
 
 
@@ -41,31 +45,37 @@ def _norm_type(norm_type) -> int:
     return p
 
 
-def _table(ctype, values):
-    return (ctype * max(len(values), 1))(*values)
-
-
 def _launch(grads: Sequence[torch.Tensor], p: int, max_norm: Optional[float], out) -> torch.Tensor:
-    device = grads[0].device
+    first = grads[0]
+    index = first.get_device()
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            return _launch(grads, p, max_norm, out)
     lib = _lib.load()
     n = len(grads)
-    src = _table(C.c_void_p, [g.data_ptr() for g in grads])
-    numel = _table(C.c_int64, [g.numel() for g in grads])
-    types = _table(C.c_int, [_lib.DTYPES[g.dtype] for g in grads])
-    with torch.cuda.device(device):
-        stream = _lib.current_stream(device)
-        nb = lib.disco_grad_norm_workspace_bytes(n)
-        ws = torch.empty(nb, dtype=torch.uint8, device=device)
-        norm = torch.empty((), dtype=torch.float32, device=device)
-        if max_norm is None:
-            _lib.check(lib.disco_grad_norm(src, numel, types, n, p, _lib.ptr(norm), _lib.ptr(ws), nb, stream), "disco_grad_norm")
-        else:
-            dst = _table(C.c_void_p, [o.data_ptr() for o in out])
-            out_types = _table(C.c_int, [_lib.DTYPES[o.dtype] for o in out])
-            status = lib.disco_grad_clip(src, dst, numel, types, out_types, n, p, max_norm, _lib.ptr(norm), _lib.ptr(ws), nb, stream)
-            if status == -1:
-                raise ValueError("clip_grads: two tensors share memory; each gradient may be scaled only once")
-            _lib.check(status, "disco_grad_clip")
+    codes = _lib.DTYPES
+    src = array("Q", [g.data_ptr() for g in grads])
+    numel = array("q", [g.numel() for g in grads])
+    types = array("i", [codes[g.dtype] for g in grads])
+    nb = lib.disco_grad_norm_workspace_bytes(n)
+    ws = torch.empty(nb, dtype=torch.uint8, device=first.device)
+    norm = torch.empty((), dtype=torch.float32, device=first.device)
+    stream = _lib.stream_of(index)
+    if max_norm is None:
+        status = lib.disco_grad_norm(src.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0], n, p, norm.data_ptr(),
+                                     ws.data_ptr(), nb, stream)
+        _lib.check(status, "disco_grad_norm")
+    else:
+        same = out is grads
+        dst = src if same else array("Q", [o.data_ptr() for o in out])
+        to = types if same else array("i", [codes[o.dtype] for o in out])
+        status = lib.disco_grad_clip(src.buffer_info()[0], dst.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0],
+                                     to.buffer_info()[0], n, p, max_norm, norm.data_ptr(), ws.data_ptr(), nb, stream)
+        if status == -1:
+            raise ValueError(_SHARED)
+        _lib.check(status, "disco_grad_clip")
+        # written behind autograd's back: whoever saved one of them must notice
+        torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
     return norm
 
 
@@ -81,7 +91,6 @@ def _dense(g: torch.Tensor) -> bool:
     return True
 
 
-@torch.no_grad()
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """``(sum |g|^p)^(1/p)`` over every element of every tensor, p = ``norm_type`` in {1, 2, inf}; a float32 scalar on the
     device.  Sums run in float64 in a fixed order: nothing overflows in between, and the result does not vary."""
@@ -90,10 +99,9 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     _on_gpu(grads)
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda" if torch.cuda.is_available() else "cpu")
-    return _launch([g if _dense(g) else g.contiguous() for g in grads], p, None, None)
+    return _launch([g if _dense(g) else g.detach().contiguous() for g in grads], p, None, None)
 
 
-@torch.no_grad()
 def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                out: Optional[Sequence[torch.Tensor]] = None, error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales every gradient by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before (float32, on the device).
@@ -113,8 +121,11 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         dst = _tensors(out)
         if len(dst) != len(grads):
             raise ValueError(f"out has {len(dst)} tensors for {len(grads)} gradients")
-        for g, o in zip(grads, dst):
-            if o.shape != g.shape or o.device != g.device or o.dtype not in (g.dtype, torch.float32):
+        if dst and dst[0].device != grads[0].device or any(
+                [o.shape != g.shape or (o.dtype != torch.float32 and o.dtype != g.dtype) for g, o in zip(grads, dst)]):
+            for g, o in zip(grads, dst):
+                if o.shape == g.shape and o.device == g.device and o.dtype in (g.dtype, torch.float32):
+                    continue
                 raise ValueError(f"out must have the gradients' shapes and device and their type or float32, got {tuple(o.shape)} "
                                  f"{o.dtype} on {o.device} for {tuple(g.shape)} {g.dtype} on {g.device}")
     _on_gpu(grads)
@@ -124,6 +135,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         norm = grad_norm(grads, norm_type)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"the norm of the gradients is {float(norm)}: they were not clipped")
+    if all([o.is_contiguous() for o in dst]) and (dst is grads or all([g.is_contiguous() for g in grads])):
+        return _launch(grads, p, max_norm, dst)
     # the kernels walk memory in order: a pair that lies differently, or with gaps, goes through contiguous copies
     src, to, back = [], [], []
     for g, o in zip(grads, dst):
@@ -132,13 +145,14 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
             to.append(o)
             continue
         if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
-            raise ValueError("clip_grads: two tensors share memory; each gradient may be scaled only once")
-        src.append(g.contiguous())
+            raise ValueError(_SHARED)
+        src.append(g.detach().contiguous())
         to.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
         back.append((o, to[-1]))
     norm = _launch(src, p, max_norm, to)
-    for o, t in back:
-        o.copy_(t)
+    with torch.no_grad():
+        for o, t in back:
+            o.copy_(t)
     return norm
 
 

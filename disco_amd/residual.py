@@ -20,58 +20,97 @@ from . import _lib
 _KINDS = {None: 0, "rms": 1, "layer": 2}
 _ACTS = {None: 0, "sigmoid": 1, "tanh": 2}
 _NO_GATE, _FULL, _ROW, _CHANNEL = 0, 1, 2, 3
+_DTYPES = _lib.DTYPES
+_F32 = torch.float32
 
 
 class _Plan:
     """What a call does besides its tensors."""
-    __slots__ = ("post", "pre", "gate", "act", "scale", "eps", "block_dtype", "param_dtype", "has_block")
+    __slots__ = ("post", "pre", "gate", "act", "scale", "eps", "block_dtype", "param_dtype", "has_block", "index")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """The tensor, or a copy, with unit column stride and rows that do not overlap (a repeated row is left as it is)."""
-    if t.shape[1] > 1 and t.stride(1) != 1 or 0 < t.stride(0) < t.shape[1] and t.shape[0] > 1 or t.stride(0) < 0:
+    if t.is_contiguous():
+        return t
+    n, F = t.shape
+    r, c = t.stride()
+    if F > 1 and c != 1 or n > 1 and 0 < r < F:
         return t.contiguous()
     return t
 
 
-def _empty(n: int, F: int, dtype, device) -> torch.Tensor:
+def _empty(x: torch.Tensor, dtype) -> torch.Tensor:
     """float32 rows start on 16 bytes, as the propagation reads them best; others lie densely."""
-    if dtype == torch.float32:
-        return torch.empty((n, (F + 3) // 4 * 4), dtype=dtype, device=device)[:, :F]
-    return torch.empty((n, F), dtype=dtype, device=device)
+    n, F = x.shape
+    if dtype == _F32 and F % 4:
+        return torch.empty((n, (F + 3) // 4 * 4), dtype=dtype, device=x.device)[:, :F]
+    return torch.empty((n, F), dtype=dtype, device=x.device)
+
+
+def _ptr(t):
+    return 0 if t is None else t.data_ptr()
 
 
 def _describe(plan, x, y, gate, scale, w1, b1, w2, b2) -> "_lib.ResidualNorm":
-    p, types = _lib.ptr, _lib.DTYPES
+    n, F = x.shape
     return _lib.ResidualNorm(
-        x.shape[0], x.shape[1], x.stride(0), 0 if y is None else y.stride(0), gate.stride(0) if gate is not None else 0,
-        p(x), p(y), p(gate), p(w1), p(b1), p(w2), p(b2), p(scale),
-        types[x.dtype], types[plan.block_dtype], types[plan.param_dtype], int(plan.has_block), plan.post, plan.pre, plan.gate, plan.act,
-        plan.scale, plan.eps)
+        n, F, x.stride(0), 0 if y is None else y.stride(0), 0 if gate is None else gate.stride(0), x.data_ptr(), _ptr(y), _ptr(gate),
+        _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(scale), _DTYPES[x.dtype], _DTYPES[plan.block_dtype], _DTYPES[plan.param_dtype],
+        plan.has_block, plan.post, plan.pre, plan.gate, plan.act, plan.scale, plan.eps)
 
 
 def _forward(plan, x, y, gate, scale, w1, b1, w2, b2, keep: bool):
-    n, F = x.shape
-    device = x.device
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        out = _empty(n, F, x.dtype, device) if plan.has_block else None
-        h = _empty(n, F, plan.block_dtype, device) if plan.pre else None
-        stats = torch.empty(4 * n, dtype=torch.float32, device=device) if keep else None
-        d = _describe(plan, x, y, gate, scale, w1, b1, w2, b2)
-        _lib.check(lib.disco_residual_norm_forward(d, _lib.ptr(out), out.stride(0) if out is not None else 0, _lib.ptr(h),
-                                                   h.stride(0) if h is not None else 0, _lib.ptr(stats), _lib.current_stream(device)),
-                   "disco_residual_norm_forward")
+    if plan.index != torch.cuda.current_device():
+        with torch.cuda.device(plan.index):
+            return _forward(plan, x, y, gate, scale, w1, b1, w2, b2, keep)
+    out = _empty(x, x.dtype) if plan.has_block else None
+    h = _empty(x, plan.block_dtype) if plan.pre else None
+    stats = torch.empty(4 * x.shape[0], dtype=_F32, device=x.device) if keep else None
+    status = _lib.load().disco_residual_norm_forward(
+        _describe(plan, x, y, gate, scale, w1, b1, w2, b2), _ptr(out), 0 if out is None else out.stride(0), _ptr(h),
+        0 if h is None else h.stride(0), _ptr(stats), _lib.stream_of(plan.index))
+    if status:
+        _lib.check(status, "disco_residual_norm_forward")
     return out, h, stats
+
+
+def _backward(plan, needs, dout, dh, x, y, gate, scale, w1, b1, w2, b2, stats):
+    if plan.index != torch.cuda.current_device():
+        with torch.cuda.device(plan.index):
+            return _backward(plan, needs, dout, dh, x, y, gate, scale, w1, b1, w2, b2, stats)
+    n, F = x.shape
+    dout = None if dout is None else _rows(dout)
+    dh = None if dh is None else _rows(dh)
+
+    def like(t, wanted):
+        return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
+
+    nx, ny, ng, ns, nw1, nb1, nw2, nb2 = needs
+    # without a gradient of h the stream's gradient is that of out itself
+    through = dh is None
+    dx = (dout if nx else None) if through else like(x, nx)
+    dy, dg, ds, dw1, db1 = like(y, ny), like(gate, ng), like(scale, ns), like(w1, nw1), like(b1, nb1)
+    dw2, db2 = (None, None) if through else (like(w2, nw2), like(b2, nb2))
+    lib = _lib.load()
+    nb = lib.disco_residual_norm_workspace_bytes(n, F)
+    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
+
+    def stride(t):
+        return F if t is None else t.stride(0)
+
+    g = _lib.ResidualNormGrads(_ptr(dout), _ptr(dh), 0 if through else _ptr(dx), _ptr(dy), _ptr(dg), stride(dout), stride(dh), stride(dx),
+                               stride(dy), stride(dg), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), _ptr(ds))
+    status = lib.disco_residual_norm_backward(_describe(plan, x, y, gate, scale, w1, b1, w2, b2), _ptr(stats), g, ws.data_ptr(), nb,
+                                              _lib.stream_of(plan.index))
+    if status:
+        _lib.check(status, "disco_residual_norm_backward")
+    return None, dx, dy, dg, ds, dw1, db1, dw2, db2
 
 
 class _ResidualNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, plan, x, y, gate, scale, w1, b1, w2, b2):
-        x = _rows(x)
-        y = None if y is None else _rows(y)
-        if plan.gate == _FULL:
-            gate = _rows(gate)
         out, h, stats = _forward(plan, x, y, gate, scale, w1, b1, w2, b2, True)
         ctx.plan = plan
         ctx.set_materialize_grads(False)
@@ -84,88 +123,81 @@ class _ResidualNormFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, *grads):
         plan = ctx.plan
-        x, y, gate, scale, w1, b1, w2, b2, stats = ctx.saved_tensors
-        dout, dh = (grads if len(grads) == 2 else (grads[0], None) if plan.has_block else (None, grads[0]))
-        _, nx, ny, ng, ns, nw1, nb1, nw2, nb2 = ctx.needs_input_grad
+        dout, dh = grads if len(grads) == 2 else (grads[0], None) if plan.has_block else (None, grads[0])
         if dout is None and dh is None:
             return (None,) * 9
-        n, F = x.shape
-        device = x.device
-        dout = None if dout is None else _rows(dout)
-        dh = None if dh is None else _rows(dh)
-        lib = _lib.load()
-        with torch.cuda.device(device):
-            def like(t, wanted):
-                return torch.empty(t.shape, dtype=t.dtype, device=device) if wanted and t is not None else None
-
-            # without a gradient of h the stream's gradient is that of out itself
-            through = dh is None and dout is not None
-            dx = dout if through and nx else like(x, nx)
-            dy, dg, ds = like(y, ny), like(gate, ng), like(scale, ns)
-            dw1, db1 = like(w1, nw1), like(b1, nb1)
-            dw2, db2 = (like(w2, nw2), like(b2, nb2)) if dh is not None else (None, None)
-            d = _describe(plan, x, y, gate, scale, w1, b1, w2, b2)
-            nb = lib.disco_residual_norm_workspace_bytes(n, F)
-            ws = torch.empty(max(int(nb), 1), dtype=torch.uint8, device=device)
-            s0 = lambda t: t.stride(0) if t is not None else F  # noqa: E731
-            p = _lib.ptr
-            g = _lib.ResidualNormGrads(p(dout), p(dh), None if through else p(dx), p(dy), p(dg), s0(dout), s0(dh), s0(dx), s0(dy),
-                                       s0(dg), p(dw1), p(db1), p(dw2), p(db2), p(ds))
-            _lib.check(lib.disco_residual_norm_backward(d, p(stats), g, p(ws), ws.numel(), _lib.current_stream(device)),
-                       "disco_residual_norm_backward")
-        return None, dx, dy, dg, ds, dw1, db1, dw2, db2
+        return _backward(plan, ctx.needs_input_grad[1:], dout, dh, *ctx.saved_tensors)
 
 
-def _check(t, what: str, shapes=None, device=None) -> None:
-    if not isinstance(t, torch.Tensor) or t.layout != torch.strided:
+def _matrix(x, what: str):
+    if not isinstance(x, torch.Tensor) or x.layout is not torch.strided:
         raise TypeError(f"{what} must be a dense tensor")
-    if shapes is not None and tuple(t.shape) not in shapes:
-        raise ValueError(f"{what} must be of shape {' or '.join(str(list(s)) for s in shapes)}, got {list(t.shape)}")
-    if device is not None and t.device != device:
-        raise RuntimeError(f"{what} is on {t.device}, x on {device}")
-
-
-def _plan(x, block_dtype, post, pre, gate_kind, gate_act, scale, eps, has_block) -> _Plan:
     if x.dim() != 2:
-        raise ValueError(f"x must be [rows, width], got {list(x.shape)}")
-    if not 1 <= x.shape[1] <= _lib.RESIDUAL_MAX_WIDTH:
-        raise ValueError(f"width {x.shape[1]} is outside 1 .. {_lib.RESIDUAL_MAX_WIDTH}")
-    if x.dtype not in _lib.DTYPES or block_dtype not in _lib.DTYPES or (x.dtype != block_dtype and x.dtype != torch.float32):
+        raise ValueError(f"{what} must be [rows, width], got {list(x.shape)}")
+    return x
+
+
+def _plan(x, block_dtype, post, pre, gate_kind, gate_act, scale, eps, has_block, vectors) -> _Plan:
+    """Checks what the tensors and options have to be, and settles the parameters' type: theirs, or float32 where they differ."""
+    F, device = x.shape[1], x.device
+    if not 1 <= F <= _lib.RESIDUAL_MAX_WIDTH:
+        raise ValueError(f"width {F} is outside 1 .. {_lib.RESIDUAL_MAX_WIDTH}")
+    if x.dtype not in _DTYPES or block_dtype not in _DTYPES or (x.dtype != block_dtype and x.dtype != _F32):
         raise TypeError(f"types are float32, float16 or bfloat16, the same for stream and block, or a float32 stream: got {x.dtype} and "
                         f"{block_dtype}")
-    for kind in (post, pre):
-        if kind not in _KINDS:
-            raise ValueError(f"a norm is 'rms', 'layer' or None, got {kind!r}")
+    if post not in _KINDS or pre not in _KINDS:
+        raise ValueError(f"a norm is 'rms', 'layer' or None, got {post!r} and {pre!r}")
     if gate_act not in _ACTS:
         raise ValueError(f"gate_act is 'sigmoid', 'tanh' or None, got {gate_act!r}")
-    if not (eps > 0.0 and math.isfinite(eps)):
+    if not 0.0 < eps < math.inf:
         raise ValueError(f"eps must be positive, got {eps}")
+    dtype = None
+    for name, v in vectors:
+        if v is None:
+            continue
+        if not isinstance(v, torch.Tensor) or v.layout is not torch.strided:
+            raise TypeError(f"{name} must be a dense tensor")
+        if v.shape != (F,):
+            raise ValueError(f"{name} must be of shape [{F}], got {list(v.shape)}")
+        if v.dtype not in _DTYPES:
+            raise TypeError(f"{name} must be float32, float16 or bfloat16, got {v.dtype}")
+        if v.device != device:
+            raise RuntimeError(f"{name} is on {v.device}, x on {device}")
+        dtype = v.dtype if dtype is None or dtype == v.dtype else _F32
+    if not x.is_cuda:
+        raise RuntimeError(f"x is on {device}: disco_amd runs on the GPU only, there is no CPU fallback")
     plan = _Plan()
     plan.post, plan.pre, plan.gate, plan.act = _KINDS[post], _KINDS[pre], gate_kind, _ACTS[gate_act]
-    plan.scale, plan.eps, plan.block_dtype, plan.has_block = float(scale), float(eps), block_dtype, has_block
+    plan.scale, plan.eps, plan.block_dtype, plan.has_block = scale, eps, block_dtype, has_block
+    plan.param_dtype, plan.index = dtype or _F32, x.get_device()
     return plan
 
 
-def _vectors(plan, x, vectors):
-    """Parameter vectors on x's device, contiguous and of one type (mixed types meet in float32)."""
-    dtypes = set()
-    for name, v in vectors.items():
+def _run(plan, x, y, gate, vectors):
+    """The call itself: tensors as the kernels read them, through autograd where one of them needs a gradient."""
+    x = _rows(x)
+    if y is not None:
+        y = _rows(y)
+    if plan.gate == _FULL:
+        gate = _rows(gate)
+    grads = torch.is_grad_enabled() and (x.requires_grad or (y is not None and y.requires_grad) or (gate is not None and gate.requires_grad))
+    dtype = plan.param_dtype
+    tensors = [x, y, gate]
+    for name, v in vectors:
         if v is not None:
-            _check(v, name, [(x.shape[1],)], x.device)
-            if v.dtype not in _lib.DTYPES:
-                raise TypeError(f"{name} must be float32, float16 or bfloat16, got {v.dtype}")
-            dtypes.add(v.dtype)
-    plan.param_dtype = dtypes.pop() if len(dtypes) == 1 else torch.float32
-    return [None if v is None else v.to(plan.param_dtype).contiguous() for v in vectors.values()]
-
-
-def _run(plan, *tensors):
-    if tensors[0].device.type != "cuda":
-        raise RuntimeError(f"x is on {tensors[0].device}: disco_amd runs on the GPU only, there is no CPU fallback")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+            grads = grads or (v.requires_grad and torch.is_grad_enabled())
+            if v.dtype != dtype:
+                v = v.to(dtype)
+            if not v.is_contiguous():
+                v = v.contiguous()
+        if name == "gate":
+            if v is not None:
+                tensors[2] = v
+        else:
+            tensors.append(v)
+    if grads:
         return _ResidualNormFn.apply(plan, *tensors)
-    x, y, gate, *vectors = (None if t is None else t.detach() for t in tensors)
-    out, h, _ = _forward(plan, _rows(x), None if y is None else _rows(y), _rows(gate) if plan.gate == _FULL else gate, *vectors, False)
+    out, h, _ = _forward(plan, *tensors, False)
     if out is None:
         return h
     return out if h is None else (out, h)
@@ -177,12 +209,11 @@ def row_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optio
 
     kind   "layer": ``(x - mean) / sqrt(var + eps) * weight + bias``; "rms": ``x / sqrt(mean(x^2) + eps) * weight + bias``
     dtype  type of the result where it is not x's: a 16-bit block on a float32 stream."""
-    _check(x, "x")
+    _matrix(x, "x")
     if kind is None:
         raise ValueError("kind is 'rms' or 'layer'")
-    plan = _plan(x, dtype or x.dtype, None, kind, _NO_GATE, None, 1.0, eps, False)
-    weight, bias = _vectors(plan, x, {"weight": weight, "bias": bias})
-    return _run(plan, x, None, None, None, None, None, weight, bias)
+    vectors = (("scale", None), ("post_weight", None), ("post_bias", None), ("weight", weight), ("bias", bias))
+    return _run(_plan(x, dtype or x.dtype, None, kind, _NO_GATE, None, 1.0, eps, False, vectors), x, None, None, vectors)
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: Optional[torch.Tensor] = None, gate_act: Optional[str] = None,
@@ -195,32 +226,38 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: Optional[torch.Tens
                stream with a 16-bit block; ``out`` has x's type, ``h`` has y's.  ``h`` is the norm of the sum before it
                is rounded to x's type.
     gate       [rows, width] or [rows, 1] (y's type), or [width] (a parameter); ``gate_act`` is "sigmoid", "tanh" or None.
-               With one row, [1, 1] is the row's gate (and so it is with a width of 1).
     scale      a number, or a vector [width] to be learned.
     post, pre  "rms", "layer" or None, each with an optional weight and bias [width] (float32 or 16-bit)."""
-    _check(x, "x")
-    if x.dim() != 2:
-        raise ValueError(f"x must be [rows, width], got {list(x.shape)}")
-    n, F = x.shape
-    _check(y, "y", [(n, F)], x.device)
-    gate_kind, vector = _NO_GATE, None
+    _matrix(x, "x")
+    _matrix(y, "y")
+    if y.shape != x.shape:
+        raise ValueError(f"y must be of x's shape {list(x.shape)}, got {list(y.shape)}")
+    if y.device != x.device:
+        raise RuntimeError(f"y is on {y.device}, x on {x.device}")
+    kind, vector, channel = _NO_GATE, None, None
     if gate is not None:
-        _check(gate, "gate", [(n, F), (n, 1), (F,)], x.device)
-        gate_kind = _CHANNEL if gate.dim() == 1 else _ROW if gate.shape[1] == 1 else _FULL
-        if gate_kind != _CHANNEL and gate.dtype != y.dtype:
-            raise TypeError(f"a gate for each row must be {y.dtype} like y, got {gate.dtype}")
+        if isinstance(gate, torch.Tensor) and gate.dim() == 1:
+            kind, channel, gate = _CHANNEL, gate, None
+        else:
+            _matrix(gate, "gate")
+            n, F = x.shape
+            if gate.shape != (n, F) and gate.shape != (n, 1):
+                raise ValueError(f"gate must be of shape [{n}, {F}], [{n}, 1] or [{F}], got {list(gate.shape)}")
+            if gate.dtype != y.dtype:
+                raise TypeError(f"a gate for each row must be {y.dtype} like y, got {gate.dtype}")
+            if gate.device != x.device:
+                raise RuntimeError(f"gate is on {gate.device}, x on {x.device}")
+            kind = _ROW if gate.shape[1] == 1 else _FULL
     elif gate_act is not None:
         raise ValueError("gate_act needs a gate")
     if isinstance(scale, torch.Tensor):
         scale, vector = 1.0, scale
-    elif not math.isfinite(scale):
+    elif not -math.inf < scale < math.inf:
         raise ValueError(f"scale must be finite, got {scale}")
     if post is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias need a post norm")
     if pre is None and (pre_weight is not None or pre_bias is not None):
         raise ValueError("pre_weight and pre_bias need a pre norm")
-    plan = _plan(x, y.dtype, post, pre, gate_kind, gate_act, scale, eps, True)
-    channel, vector, w1, b1, w2, b2 = _vectors(plan, x, {"gate": gate if gate_kind == _CHANNEL else None, "scale": vector,
-                                                        "post_weight": post_weight, "post_bias": post_bias, "pre_weight": pre_weight,
-                                                        "pre_bias": pre_bias})
-    return _run(plan, x, y, channel if gate_kind == _CHANNEL else gate, vector, w1, b1, w2, b2)
+    vectors = (("gate", channel), ("scale", vector), ("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
+               ("pre_bias", pre_bias))
+    return _run(_plan(x, y.dtype, post, pre, kind, gate_act, scale, eps, True, vectors), x, y, gate, vectors)
