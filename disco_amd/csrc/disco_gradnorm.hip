@@ -3,8 +3,8 @@
 //   norm = (sum over every element of every tensor |g|^p)^(1/p), p = 1, 2 or infinity
 //   out  = g * min(1, max_norm / (norm + 1e-6))
 //
-// Bound by memory: the norm reads every gradient once, clipping reads it again (no element may be scaled before the last
-// one has been read) and writes it once.  The tensors are named in the launch's own arguments, up to a few hundred per
+// Bound by memory: the norm reads every gradient once (201 M float32 values: 141 us, 5.7 TB/s), clipping reads it again, since
+// no element may be scaled before the last one has been read, and writes it once.  The tensors are named in the launch's own arguments, up to a few hundred per
 // launch, so that no table is copied to the device and a launch can be captured.  Sums are float64 per lane: squares of
 // float32 values neither overflow nor vanish there, and one conversion and one fused add per element cost nothing next to
 // the read.  Every sum has a fixed order: the norm is the same from run to run.
@@ -20,22 +20,18 @@
 
 namespace disco {
 
-constexpr int kChunk = 4096;             // elements a workgroup takes at a time
-constexpr int kNormTensors = 190;        // tensors named by one launch: its arguments stay below 4 KiB
-constexpr int kClipTensors = 136;
-constexpr int kMostGroups = 2048;        // workgroups of one launch: eight per compute unit
+// of a tensor, that a workgroup takes at a time: four loads of 16 bytes a lane (with two, bfloat16 came in at 4.4 TB/s
+// instead of 5.2)
+constexpr int kChunkBytes = 16384;
+constexpr int kTensors = 136;            // tensors named by one launch: its arguments stay below 4 KiB
+constexpr int kGroups = 8192;            // workgroups of one launch of the norm, at most
+constexpr int kJoin = 2048;              // partial sums that every workgroup of the clipping joins for itself
 
-template <int MOST> struct NormTable {
-  const void* src[MOST];
-  int64_t numel[MOST];
-  uint32_t end[MOST];                    // chunks up to and including this tensor
-  int count;
-};
-template <int MOST> struct ClipTable {
-  const void* src[MOST];
-  void* dst[MOST];
-  int64_t numel[MOST];
-  uint32_t end[MOST];
+struct Table {
+  const void* src[kTensors];
+  void* dst[kTensors];
+  int64_t numel[kTensors];
+  uint32_t end[kTensors];                // chunks up to and including this tensor
   int count;
 };
 
@@ -50,28 +46,30 @@ template <int P> __device__ __forceinline__ double norm_join(double s, double t)
   return (t > s || t != t) ? t : s;
 }
 
-// fixed-order sum over the workgroup's 256 lanes, in every lane
-template <int P> __device__ __forceinline__ double norm_block(double s, double* lds) {
+// fixed-order sum over the workgroup's lanes, in every lane
+template <int P, int WAVES> __device__ __forceinline__ double norm_block(double s, double* lds) {
   for (int o = 32; o > 0; o >>= 1) s = norm_join<P>(s, __shfl_xor(s, o, 64));
-  __syncthreads();
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
   __syncthreads();
-  return norm_join<P>(norm_join<P>(lds[0], lds[1]), norm_join<P>(lds[2], lds[3]));
+  s = lds[0];
+#pragma unroll
+  for (int w = 1; w < WAVES; ++w) s = norm_join<P>(s, lds[w]);
+  return s;
 }
 
 // the chunks [first, last) of a workgroup: contiguous, so that the table is searched once
-__device__ __forceinline__ void share(uint32_t chunks, uint32_t& first, uint32_t& last) {
-  first = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x);
-  last = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
+__device__ __forceinline__ void share(uint32_t chunks, uint32_t index, uint32_t& first, uint32_t& last) {
+  first = (uint32_t)((uint64_t)chunks * index / gridDim.x);
+  last = (uint32_t)((uint64_t)chunks * (index + 1) / gridDim.x);
 }
 
 template <typename T, int P>
-__global__ __launch_bounds__(256) void k_norm_partial(const NormTable<kNormTensors> t, double* __restrict__ partial) {
+__global__ __launch_bounds__(256) void k_norm_partial(const Table t, double* __restrict__ partial) {
   typedef T vec __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T))));
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), kChunk = kChunkBytes / sizeof(T);
   __shared__ double lds[4];
   uint32_t chunk, last;
-  share(t.end[t.count - 1], chunk, last);
+  share(t.end[t.count - 1], blockIdx.x, chunk, last);
   int k = 0;
   for (int lo = 0, hi = t.count - 1; lo <= hi;) {      // first tensor whose end lies behind the chunk
     const int mid = (lo + hi) >> 1;
@@ -95,45 +93,51 @@ __global__ __launch_bounds__(256) void k_norm_partial(const NormTable<kNormTenso
       for (int i = threadIdx.x; i < (int)left; i += 256) s = norm_add<P>(s, (float)p[i]);
     }
   }
-  s = norm_block<P>(s, lds);
+  s = norm_block<P, 4>(s, lds);
   if (threadIdx.x == 0) partial[blockIdx.x] = s;
 }
 
-template <int P> __device__ __forceinline__ double norm_total(const double* __restrict__ partial, int groups, double* lds) {
+template <int P, int WAVES> __device__ __forceinline__ double norm_total(const double* __restrict__ partial, int64_t groups, double* lds) {
   double s = 0.0;
-  for (int i = threadIdx.x; i < groups; i += 256) s = norm_join<P>(s, partial[i]);
-  s = norm_block<P>(s, lds);
-  return P == 2 ? sqrt(s) : s;
+  for (int64_t i = threadIdx.x; i < groups; i += WAVES * 64) s = norm_join<P>(s, partial[i]);
+  return norm_block<P, WAVES>(s, lds);
 }
 
-template <int P> __global__ __launch_bounds__(256) void k_norm_finish(const double* __restrict__ partial, int groups, float* __restrict__ norm) {
-  __shared__ double lds[4];
-  const double s = norm_total<P>(partial, groups, lds);
-  if (threadIdx.x == 0) *norm = (float)s;
+template <int P>
+__global__ __launch_bounds__(1024) void k_norm_finish(const double* __restrict__ partial, int64_t groups, double* __restrict__ joined,
+                                                      float* __restrict__ norm) {
+  __shared__ double lds[16];
+  const double s = norm_total<P, 16>(partial, groups, lds);
+  if (threadIdx.x == 0) {
+    if (joined) *joined = s;
+    if (norm) *norm = (float)(P == 2 ? sqrt(s) : s);
+  }
 }
 
 template <typename T, typename U, int P>
-__global__ __launch_bounds__(256) void k_clip(const ClipTable<kClipTensors> t, const double* __restrict__ partial, int groups,
+__global__ __launch_bounds__(256) void k_clip(const Table t, const double* __restrict__ partial, int64_t groups,
                                               double max_norm, float* __restrict__ norm) {
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), kChunk = kChunkBytes / sizeof(T);
   typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
   typedef U uvec __attribute__((ext_vector_type(V), aligned(sizeof(U))));
   __shared__ double lds[4];
   // every workgroup joins the partial sums for itself, in the same order: no launch in between
-  const double total = norm_total<P>(partial, groups, lds);
+  const double sum = norm_total<P, 4>(partial, groups, lds), total = P == 2 ? sqrt(sum) : sum;
   if (norm && blockIdx.x == 0 && threadIdx.x == 0) *norm = (float)total;
   const double want = max_norm / (total + 1e-6);
   // float64 like the norm: beside gradients near float32's end the factor is no normal float32.  A NaN norm stays NaN.
   const double factor = want >= 1.0 ? 1.0 : want;
-  uint32_t chunk, last;
-  share(t.end[t.count - 1], chunk, last);
-  int k = 0;
-  for (int lo = 0, hi = t.count - 1; lo <= hi;) {
+  // from the end: what the norm read last still lies in the last-level cache
+  uint32_t first, chunk;
+  share(t.end[t.count - 1], gridDim.x - 1 - blockIdx.x, first, chunk);
+  int k = t.count - 1;
+  for (int lo = 0, hi = t.count - 1; lo <= hi;) {      // first tensor whose end lies at the share's end or behind it
     const int mid = (lo + hi) >> 1;
-    if (t.end[mid] > chunk) { k = mid; hi = mid - 1; } else lo = mid + 1;
+    if (t.end[mid] >= chunk) { k = mid; hi = mid - 1; } else lo = mid + 1;
   }
-  for (; chunk < last; ++chunk) {
-    while (t.end[k] <= chunk) ++k;
+  while (chunk > first) {
+    --chunk;
+    while (k > 0 && t.end[k - 1] > chunk) --k;
     if (factor == 1.0 && t.src[k] == t.dst[k]) continue;      // in place and within the norm: nothing changes
     const int64_t at = (int64_t)(chunk - (k ? t.end[k - 1] : 0)) * kChunk;
     const int64_t left = t.numel[k] - at;
@@ -181,27 +185,13 @@ static bool overlap(const std::vector<Item>& items) {
   return false;
 }
 
-static int64_t chunks_of(const Item& i) { return (i.numel + kChunk - 1) / kChunk; }
+static int64_t chunks_of(const Item& i) { return (i.numel * size_of(i.type) + kChunkBytes - 1) / kChunkBytes; }
 
-// Workgroups of the launches: what their chunks need, 2048 together at most, but at least 8 each.
-static int64_t groups_of(int64_t chunks, int64_t all) {
-  const int64_t part = all > kMostGroups ? std::max<int64_t>(8, chunks * kMostGroups / all) : chunks;
-  return std::min(chunks, part);
-}
-
-// items of one type pair [b, e) -> launches of at most `most` tensors and 2^31 chunks
-template <typename F> static int cut(const std::vector<Item>& items, size_t b, size_t e, int most, F&& launch) {
-  while (b < e) {
-    size_t c = b;
-    int64_t chunks = 0;
-    while (c < e && (int)(c - b) < most && chunks + chunks_of(items[c]) < ((int64_t)1 << 31)) chunks += chunks_of(items[c++]);
-    if (c == b) return DISCO_EUNSUPPORTED;      // one tensor of 2^31 chunks: 16 TB
-    const int rc = launch(b, c, chunks);
-    if (rc != DISCO_OK) return rc;
-    b = c;
-  }
-  return DISCO_OK;
-}
+static int64_t norm_groups(int64_t chunks) { return std::min<int64_t>(chunks, kGroups); }
+// A workgroup for each chunk (up to 2^20), rather than few that walk far apart: they are dealt out in order, so memory is read
+// and written in few places at a time (1.2 G values, bfloat16 to float32: 1.36 ms, with 16384 workgroups 1.49, with 2048 1.67,
+// with 512 2.01).
+static int64_t clip_groups(int64_t chunks) { return std::min<int64_t>(chunks, 1 << 20); }
 
 template <typename F> static int by_type(int type, F&& f) {
   return type == DISCO_F32 ? f(float{}) : type == DISCO_F16 ? f(_Float16{}) : f(__bf16{});
@@ -210,79 +200,90 @@ template <typename F> static int by_norm(int norm_type, F&& f) {
   return norm_type == 2 ? f(std::integral_constant<int, 2>{}) : norm_type == 1 ? f(std::integral_constant<int, 1>{}) : f(std::integral_constant<int, 0>{});
 }
 
+struct Launch { size_t from, to; int64_t chunks; };
+
+// runs of one type pair, cut where the table or the chunks' numbers end
+static int cut(const std::vector<Item>& items, std::vector<Launch>* launches) {
+  for (size_t b = 0; b < items.size();) {
+    Launch l{b, b, 0};
+    while (l.to < items.size() && l.to - b < (size_t)kTensors && items[l.to].type == items[b].type && items[l.to].out_type == items[b].out_type &&
+           l.chunks + chunks_of(items[l.to]) < ((int64_t)1 << 31))
+      l.chunks += chunks_of(items[l.to++]);
+    if (l.to == b) return DISCO_EUNSUPPORTED;      // one tensor of 2^31 chunks: 32 TB
+    launches->push_back(l);
+    b = l.to;
+  }
+  return DISCO_OK;
+}
+
+static void fill(const std::vector<Item>& items, const Launch& l, Table* t) {
+  uint32_t end = 0;
+  t->count = (int)(l.to - l.from);
+  for (size_t i = l.from; i < l.to; ++i) {
+    t->src[i - l.from] = items[i].src;
+    t->dst[i - l.from] = items[i].dst;
+    t->numel[i - l.from] = items[i].numel;
+    t->end[i - l.from] = end += (uint32_t)chunks_of(items[i]);
+  }
+}
+
 static int gradient_norm(std::vector<Item>& items, int norm_type, bool clip, double max_norm, float* norm, void* ws, size_t ws_bytes,
                          hipStream_t stream) {
   double* partial = static_cast<double*>(ws);
   const int64_t room = (int64_t)(ws_bytes / sizeof(double));
   std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.type != b.type ? a.type < b.type : a.out_type < b.out_type; });
-  int64_t all = 0, groups = 0;
-  for (const Item& i : items) all += chunks_of(i);
-  auto ranges = [&](bool both, auto&& f) -> int {
-    for (size_t b = 0; b < items.size();) {
-      size_t e = b;
-      while (e < items.size() && items[e].type == items[b].type && (!both || items[e].out_type == items[b].out_type)) ++e;
-      const int rc = f(b, e);
-      if (rc != DISCO_OK) return rc;
-      b = e;
-    }
-    return DISCO_OK;
-  };
-  int rc = ranges(false, [&](size_t b, size_t e) -> int {
-    return cut(items, b, e, kNormTensors, [&](size_t from, size_t to, int64_t chunks) -> int {
-      NormTable<kNormTensors> t;
-      uint32_t end = 0;
-      t.count = (int)(to - from);
-      for (size_t i = from; i < to; ++i) {
-        t.src[i - from] = items[i].src;
-        t.numel[i - from] = items[i].numel;
-        t.end[i - from] = end += (uint32_t)chunks_of(items[i]);
-      }
-      const int64_t g = groups_of(chunks, all);
-      if (groups + g > room) return DISCO_EWORKSPACE;
-      const int r = by_type(items[from].type, [&](auto v) -> int {
-        return by_norm(norm_type, [&](auto p) -> int {
-          hipLaunchKernelGGL((k_norm_partial<decltype(v), decltype(p)::value>), dim3((unsigned)g), dim3(256), 0, stream, t, partial + groups);
-          DISCO_CHECK_LAUNCH();
-          return DISCO_OK;
-        });
-      });
-      groups += g;
-      return r;
-    });
-  });
+  std::vector<Launch> launches;
+  const int rc = cut(items, &launches);
   if (rc != DISCO_OK) return rc;
-  if (!clip || items.empty())
-    return by_norm(norm_type, [&](auto p) -> int {
-      hipLaunchKernelGGL((k_norm_finish<decltype(p)::value>), dim3(1), dim3(256), 0, stream, partial, (int)groups, norm);
+  int64_t groups = 0;
+  for (const Launch& l : launches) groups += norm_groups(l.chunks);
+  if (groups + 1 > room) return DISCO_EWORKSPACE;
+  Table t;
+  int64_t at = 0;
+  for (const Launch& l : launches) {
+    fill(items, l, &t);
+    const int64_t g = norm_groups(l.chunks);
+    const int r = by_type(items[l.from].type, [&](auto v) -> int {
+      return by_norm(norm_type, [&](auto p) -> int {
+        hipLaunchKernelGGL((k_norm_partial<decltype(v), decltype(p)::value>), dim3((unsigned)g), dim3(256), 0, stream, t, partial + at);
+        DISCO_CHECK_LAUNCH();
+        return DISCO_OK;
+      });
+    });
+    if (r != DISCO_OK) return r;
+    at += g;
+  }
+  const bool only = !clip || items.empty();
+  if (only || groups > kJoin) {
+    const int r = by_norm(norm_type, [&](auto p) -> int {
+      hipLaunchKernelGGL((k_norm_finish<decltype(p)::value>), dim3(1), dim3(1024), 0, stream, partial, groups, only ? nullptr : partial + groups,
+                         only ? norm : nullptr);
       DISCO_CHECK_LAUNCH();
       return DISCO_OK;
     });
-  return ranges(true, [&](size_t b, size_t e) -> int {
-    return cut(items, b, e, kClipTensors, [&](size_t from, size_t to, int64_t chunks) -> int {
-      ClipTable<kClipTensors> t;
-      uint32_t end = 0;
-      t.count = (int)(to - from);
-      for (size_t i = from; i < to; ++i) {
-        t.src[i - from] = items[i].src;
-        t.dst[i - from] = items[i].dst;
-        t.numel[i - from] = items[i].numel;
-        t.end[i - from] = end += (uint32_t)chunks_of(items[i]);
-      }
-      const int64_t g = groups_of(chunks, all);
-      float* to_norm = from == 0 ? norm : nullptr;
-      return by_type(items[from].type, [&](auto v) -> int {
-        return by_norm(norm_type, [&](auto p) -> int {
-          auto launch = [&](auto u) -> int {
-            hipLaunchKernelGGL((k_clip<decltype(v), decltype(u), decltype(p)::value>), dim3((unsigned)g), dim3(256), 0, stream, t, partial,
-                               (int)groups, max_norm, to_norm);
-            DISCO_CHECK_LAUNCH();
-            return DISCO_OK;
-          };
-          return items[from].out_type == DISCO_F32 ? launch(float{}) : launch(v);
-        });
+    if (r != DISCO_OK || only) return r;
+    partial += groups;
+    groups = 1;
+  }
+  for (size_t i = launches.size(); i-- > 0;) {
+    const Launch& l = launches[i];
+    if (launches.size() > 1) fill(items, l, &t);
+    const int64_t g = clip_groups(l.chunks);
+    float* to = i == 0 ? norm : nullptr;
+    const int r = by_type(items[l.from].type, [&](auto v) -> int {
+      return by_norm(norm_type, [&](auto p) -> int {
+        auto launch = [&](auto u) -> int {
+          hipLaunchKernelGGL((k_clip<decltype(v), decltype(u), decltype(p)::value>), dim3((unsigned)g), dim3(256), 0, stream, t, partial,
+                             groups, max_norm, to);
+          DISCO_CHECK_LAUNCH();
+          return DISCO_OK;
+        };
+        return items[l.from].out_type == DISCO_F32 ? launch(float{}) : launch(v);
       });
     });
-  });
+    if (r != DISCO_OK) return r;
+  }
+  return DISCO_OK;
 }
 
 static int collect(const void* const* src, void* const* dst, const int64_t* numel, const int* type, const int* out_type, int64_t n,
@@ -306,9 +307,8 @@ using namespace disco;
 
 extern "C" size_t disco_grad_norm_workspace_bytes(int64_t n_tensors) {
   if (n_tensors < 0) return 0;
-  // at most 2048 groups in proportion to the chunks, 8 for each launch that is rounded up; a launch is cut at 190 tensors,
-  // at a change of type (twice) and at 2^31 chunks
-  return (size_t)(kMostGroups + 8 * (n_tensors / kNormTensors + 4 + 8)) * sizeof(double);
+  // launches are cut at 136 tensors, where one of the five type pairs ends, and at 2^31 chunks (32 TB); their joined sum
+  return ((size_t)kGroups * (size_t)(n_tensors / kTensors + 5 + 1) + 1) * sizeof(double);
 }
 
 extern "C" int disco_grad_norm(const void* const* grads_host, const int64_t* numel_host, const int* type_host, int64_t n_tensors,
