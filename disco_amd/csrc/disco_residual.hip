@@ -33,7 +33,7 @@ struct FinishArgs {
 // float64 in a fixed order.  With c = act(channel gate) and s the scale, z = u1 * w1 + b1 gives
 //   dw1 = s c P1,  db1 = s c P2,  ds = c (w1 P1 + b1 P2),  dgate = s c' (w1 P1 + b1 P2),  dw2 = P3,  db2 = P4.
 __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
-  __shared__ double part[4][64][16];
+  __shared__ double part[4][16][16];
   const int cl = threadIdx.x & 15, slice = threadIdx.x >> 4;
   const int c = blockIdx.x * 16 + cl;
   double w = 1.0, b = 0.0, scale = (double)a.scale, g = 0.0;      // read while the sums come in
@@ -49,28 +49,32 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
     const float* p = a.partial + (int64_t)slice * 4 * a.width + c;
     const int64_t step = 64 * 4 * (int64_t)a.width;
     for (int64_t g = slice; g < a.groups; g += 64 * 4, p += 4 * step) {
-      float v[4][4];
+      float v[4][4] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 4; ++k)
+        if (a.partials >> k & 1)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[i][k] = (a.partials >> k & 1) && g + 64 * i < a.groups ? p[i * step + (int64_t)k * a.width] : 0.0f;
+          for (int i = 0; i < 4; ++i) v[k][i] = p[(g + 64 * i < a.groups ? i * step : 0) + (int64_t)k * a.width];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < 4; ++k)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) s[k] += (double)v[i][k];
+        for (int i = 0; i < 4; ++i) s[k] += g + 64 * i < a.groups ? (double)v[k][i] : 0.0;
     }
   }
+  // the four slices of a wave, then the 16 waves: lane 16 k + column of the first wave ends with sum k of its column
 #pragma unroll
-  for (int k = 0; k < 4; ++k) part[k][slice][cl] = s[k];
-  __syncthreads();
-  for (int o = 32; o > 0; o >>= 1) {
-    if (slice < o)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) part[k][slice][cl] += part[k][slice + o][cl];
-    __syncthreads();
+  for (int k = 0; k < 4; ++k) {
+    s[k] += __shfl_xor(s[k], 16, 64);
+    s[k] += __shfl_xor(s[k], 32, 64);
+    if ((threadIdx.x & 63) < 16) part[k][threadIdx.x >> 6][cl] = s[k];
   }
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) sum += part[threadIdx.x >> 4][i][cl];
+  const double P1 = __shfl(sum, cl, 64), P2 = __shfl(sum, 16 + cl, 64), P3 = __shfl(sum, 32 + cl, 64), P4 = __shfl(sum, 48 + cl, 64);
   if (slice != 0 || c >= a.width) return;
-  const double P1 = part[0][0][cl], P2 = part[1][0][cl];
   double gate = 1.0, slope = 0.0;
   if (a.channel) {
     if (a.act == DISCO_ACT_SIGMOID) { gate = 1.0 / (1.0 + exp(-g)); slope = gate * (1.0 - gate); }
@@ -82,8 +86,8 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   const double T = w * P1 + b * P2;
   if (a.dlam) param_put(a.dlam, a.param_type, c, (double)a.scale * gate * T);
   if (a.channel && a.dg) param_put(a.dg, a.param_type, c, scale * slope * T);
-  if (a.dw2) param_put(a.dw2, a.param_type, c, part[2][0][cl]);
-  if (a.db2) param_put(a.db2, a.param_type, c, part[3][0][cl]);
+  if (a.dw2) param_put(a.dw2, a.param_type, c, P3);
+  if (a.db2) param_put(a.db2, a.param_type, c, P4);
 }
 
 static int pair_of(int stream_type, int block_type) {
