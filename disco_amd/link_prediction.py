@@ -79,9 +79,10 @@ def negative_sampling(edge_index: torch.Tensor, num_nodes: int, num_neg_samples:
 def link_prediction(pge_edge, feat_transform: torch.Tensor, edge_index: torch.Tensor, nedges: int, epochs: int,
                     lr: float = 0.001, neg_edge_index: Optional[torch.Tensor] = None, num_nodes: Optional[int] = None,
                     generator: Optional[torch.Generator] = None, log_every: int = 100,
-                    on_best: Optional[Callable] = None, verbose: bool = False):
+                    on_best: Optional[Callable] = None, verbose: bool = False, max_norm: Optional[float] = None):
     """The training loop of /root/reference/LargeScaleCondensing.py:176-214 with the batch assembled on the
-    device.  Returns ``(best_accuracy, last_loss)``; ``on_best(pge_edge, accuracy)`` replaces the
+    device.  ``max_norm`` clips the norm over all of the scorer's gradients in front of each step (the reference does
+    not).  Returns ``(best_accuracy, last_loss)``; ``on_best(pge_edge, accuracy)`` replaces the
     reference's ``torch.save`` of the best state_dict (:208-213)."""
     dev = feat_transform.device
     n = int(num_nodes if num_nodes is not None else feat_transform.shape[0])
@@ -89,7 +90,8 @@ def link_prediction(pge_edge, feat_transform: torch.Tensor, edge_index: torch.Te
     if neg_edge_index is None:
         neg_edge_index = negative_sampling(edge_index, n, 3 * edge_index.shape[1], generator)    # :178
     neg_edge_index = neg_edge_index.to(dev)
-    optimizer = torch.optim.Adam(pge_edge.parameters(), lr=lr)                                     # :148
+    params = list(pge_edge.parameters())
+    optimizer = torch.optim.Adam(params, lr=lr)                                     # :148
     w = feat_transform.shape[1]
     batch = torch.empty((4 * nedges, 2 * w), dtype=torch.float32, device=dev)
     y = torch.cat([torch.ones(nedges, device=dev), torch.zeros(3 * nedges, device=dev)])          # :193
@@ -105,6 +107,8 @@ def link_prediction(pge_edge, feat_transform: torch.Tensor, edge_index: torch.Te
         pred = pge_edge.forward(batch)                                                             # :196
         loss = F.binary_cross_entropy(pred, y)                                                     # :197-198
         loss.backward()
+        if max_norm is not None:
+            ops.clip_grad_norm_(params, max_norm)
         optimizer.step()
         if log_every and i % log_every == 0:                                                       # :202-214
             acc = float((torch.round(pred) == y).float().mean())

@@ -11,6 +11,10 @@ the reference (``convs.{i}.lin.weight``, ``convs.{i}.bias``, ``norms.{i}.*``, ``
 On MI355X the graph stays resident: ``predict(x, adj)`` with a device-resident ``adj`` re-uploads nothing
 (the reference ships CSR + X to the GPU for each of its 31 evaluations, LargeScaleCondensing.py:344),
 and ``full_inference`` replaces the sampler round trips of ``large_inference`` by full-graph propagation.
+
+``residual=True`` (or a dict of ``ResidualNorm`` arguments) makes every hidden layer behind the first a residual block: the
+first layer opens the stream, each further one reads its norm and is joined to it, the last reads the last norm.  Not in the
+reference; without it nothing changes.
 """
 from __future__ import annotations
 
@@ -23,6 +27,7 @@ from torch import Tensor
 from torch.nn import Linear, ModuleList
 
 from .convs_large import GCNConv, GINConv, SAGEConv, SGConv
+from .residual import ResidualNorm, RowNorm
 
 _ACTS = {"relu": torch.nn.ReLU, "elu": torch.nn.ELU, "leaky_relu": torch.nn.LeakyReLU, "tanh": torch.nn.Tanh,
          "sigmoid": torch.nn.Sigmoid, "gelu": torch.nn.GELU, "prelu": torch.nn.PReLU}
@@ -99,8 +104,10 @@ class BasicGNN(torch.nn.Module):
     def __init__(self, nfeat: int, nhid: int, nlayers: int, nclass: Optional[int] = None, dropout: float = 0.0,
                  act: Union[str, Callable, None] = "relu", act_first: bool = False, act_kwargs: Optional[Dict[str, Any]] = None,
                  norm: Union[str, Callable, None] = None, norm_kwargs: Optional[Dict[str, Any]] = None,
-                 jk: Optional[str] = None, sgc: bool = False, **kwargs):
+                 jk: Optional[str] = None, sgc: bool = False, residual: Union[bool, Dict[str, Any]] = False, **kwargs):
         super().__init__()
+        if residual is not False and (sgc or jk is not None or norm is not None or nclass is None or nlayers < 3):
+            raise ValueError("residual blocks need three layers or more and an output width, and replace norm, jk and sgc")
         self.nfeat, self.nhid = nfeat, nhid
         self.temp_layers = nlayers                      # basicgnn_large.py:80-85: SGC is ONE conv with K = nlayers
         self.nlayers = 1 if sgc else nlayers
@@ -137,6 +144,11 @@ class BasicGNN(torch.nn.Module):
             self.jk = JumpingKnowledge(jk, nhid, nlayers)
         if jk is not None:
             self.lin = Linear(nlayers * nhid if jk == "cat" else nhid, self.nclass)
+        self.residual = residual is not False
+        if self.residual:
+            config = {} if residual is True else dict(residual)
+            self.joins = ModuleList(ResidualNorm(nhid, **config) for _ in range(nlayers - 2))
+            self.first_norm = RowNorm(nhid, self.joins[0].pre.kind, self.joins[0].eps)
 
     def init_conv(self, nfeat, nclass, **kwargs):
         raise NotImplementedError
@@ -150,6 +162,30 @@ class BasicGNN(torch.nn.Module):
             self.jk.reset_parameters()
         if hasattr(self, "lin"):
             self.lin.reset_parameters()
+        if self.residual:
+            self.first_norm.reset_parameters()
+            for join in self.joins:
+                join.reset_parameters()
+
+    def _residual_layer(self, depth: int, x: Tensor, h: Tensor, conv: Callable[[Tensor], Tensor], normalise: bool = True):
+        """One depth of a residual network: from the stream ``x`` and this depth's input ``h`` to the next ones.  ``conv``
+        applies the convolution and may return fewer rows than it reads (sampled targets come first).  At the last depth the
+        second result is the output; without ``normalise`` it is None before."""
+        y = conv(h)
+        if depth == self.nlayers - 1:
+            return x, y
+        if self.act is not None:
+            y = self.act(y)
+        y = F.dropout(y, p=self.dropout, training=self.training)
+        if depth == 0:
+            return y, self.first_norm(y) if normalise else None
+        n = y.shape[0]
+        r = self.joins[depth - 1](x[:n], y, h[:n], normalise)
+        return r if normalise else (r, None)
+
+    def _block_norm(self, depth: int) -> RowNorm:
+        """The norm in front of the convolution of a depth behind the first."""
+        return self.first_norm if depth == 1 else self.joins[depth - 2].pre
 
     def _post(self, x: Tensor, i: int) -> Tensor:
         if self.act is not None and self.act_first:
@@ -162,6 +198,11 @@ class BasicGNN(torch.nn.Module):
 
     def forward(self, x: Tensor, edge_index, *, edge_weight: Optional[Tensor] = None, edge_attr=None) -> Tensor:
         # basicgnn_large.py:161-207
+        if self.residual:
+            h = x
+            for i in range(self.nlayers):
+                x, h = self._residual_layer(i, x, h, lambda v: self.convs[i](v, edge_index, edge_weight=edge_weight))
+            return F.log_softmax(h, dim=1)
         xs: List[Tensor] = []
         for i in range(self.nlayers):
             x = self.convs[i](x, edge_index, edge_weight=edge_weight)
@@ -183,6 +224,10 @@ class BasicGNN(torch.nn.Module):
         dropout; the result is log-probabilities."""
         if self.sgc:
             h = self.convs[0].forward_sampler(x, adjs)
+        elif self.residual:
+            h = x
+            for depth, hop in enumerate(adjs):
+                x, h = self._residual_layer(depth, x, h, lambda v: self.convs[depth](v, hop[0]))
         else:
             h, last = x, self.nlayers - 1
             for depth, hop in enumerate(adjs):
@@ -210,6 +255,10 @@ class BasicGNN(torch.nn.Module):
             conv = self.convs[0]
             h = conv.propagate(adj_t, x=x)[:keep]
             return conv.lin(h) if depth == self.temp_layers - 1 else h
+        if self.residual:       # the stream goes from depth to depth; each reads its norm of it
+            h = x if depth == 0 else self._block_norm(depth)(x)
+            out, y = self._residual_layer(depth, x, h, lambda v: self.convs[depth](v, adj_t)[:keep], normalise=False)
+            return out if y is None else y
         h = self.convs[depth](x, adj_t)[:keep]
         final = depth == self.nlayers - 1
         if final and raw_final:

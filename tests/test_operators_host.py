@@ -153,3 +153,28 @@ def test_gradient_entries_refuse():
     assert clip(dst=(8192, 4096)) == -1 and clip(dst=(4100, 8192)) == -1
     assert clip(types=(1, 1), to=(0, 1)) == -1                             # in place with a wider type
     assert clip(src=(4096, 4096), dst=(16384, 32768)) == -3                # read twice, written apart: allowed
+
+
+def test_residual_models_refuse_and_leave_the_others_alone():
+    from disco_amd.models import basicgnn_large as M
+    from disco_amd.models.residual import ResidualNorm, RowNorm
+    kw = dict(nfeat=6, nhid=8, nclass=3)
+    for bad in (dict(nlayers=2), dict(nlayers=4, norm="BatchNorm"), dict(nlayers=4, jk="cat"), dict(nlayers=4, nclass=None)):
+        with pytest.raises(ValueError):
+            M.GCN(residual=True, **{**kw, **bad})
+    with pytest.raises(ValueError):
+        M.SGC(nlayers=3, sgc=True, residual=True, **kw)
+    for bad in (dict(gate="edge"), dict(post="batch"), dict(pre="batch"), dict(pre=None)):
+        with pytest.raises(ValueError):
+            M.GCN(nlayers=4, residual=bad, **kw)
+    with pytest.raises(ValueError):
+        RowNorm(8, "batch")
+    plain = M.GCN(nlayers=4, **kw)
+    assert not any(k.startswith(("joins", "first_norm")) for k in plain.state_dict())
+    keys = set(M.GCN(nlayers=4, residual=dict(gate="node", learn_scale=True, post="rms"), **kw).state_dict())
+    assert keys - set(plain.state_dict()) == {"first_norm.weight", "first_norm.bias"} | {
+        f"joins.{i}.{k}" for i in range(2) for k in ("post.weight", "pre.weight", "pre.bias", "scale", "gate.weight", "gate.bias")}
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        ResidualNorm(8)(torch.zeros(4, 8), torch.zeros(4, 8), torch.zeros(4, 8))
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        RowNorm(8)(torch.zeros(4, 8))
