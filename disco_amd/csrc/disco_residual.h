@@ -43,7 +43,7 @@ enum ResidualPair { kPairF32 = 0, kPairF16 = 1, kPairBF16 = 2, kPairF32F16 = 3, 
 // bits take eight elements a lane where float32 takes four, and half the lanes: the same bytes in flight for each wave
 // (HALVES).
 struct ResidualShape { int lanes, elems; };
-constexpr ResidualShape kResidualShapes[] = {{16, 4}, {32, 4}, {64, 4}, {64, 8}, {64, 12}, {64, 16}, {128, 12},
+constexpr ResidualShape kResidualShapes[] = {{4, 4}, {8, 4}, {16, 4}, {32, 4}, {64, 4}, {64, 8}, {64, 12}, {64, 16}, {128, 12},
                                              {256, 8}, {256, 12}, {256, 16}, {512, 12}, {512, 16}, {1024, 16}};
 constexpr ResidualShape residual_shape(int64_t width, bool halves) {
   for (const ResidualShape& s : kResidualShapes)
@@ -187,10 +187,12 @@ template <int LANES, int R>
 __device__ __forceinline__ void row_sum(float (&v)[R], float4* lds, int& turn) {
 #pragma unroll
   for (int r = 0; r < R; ++r) v[r] = add_dpp<0xB1>(v[r]);       // quad_perm [1, 0, 3, 2]
+  if constexpr (LANES >= 4)
 #pragma unroll
-  for (int r = 0; r < R; ++r) v[r] = add_dpp<0x4E>(v[r]);       // quad_perm [2, 3, 0, 1]
+    for (int r = 0; r < R; ++r) v[r] = add_dpp<0x4E>(v[r]);     // quad_perm [2, 3, 0, 1]
+  if constexpr (LANES >= 8)
 #pragma unroll
-  for (int r = 0; r < R; ++r) v[r] = add_dpp<0x141>(v[r]);      // row_half_mirror
+    for (int r = 0; r < R; ++r) v[r] = add_dpp<0x141>(v[r]);    // row_half_mirror
   if constexpr (LANES >= 16)
 #pragma unroll
     for (int r = 0; r < R; ++r) v[r] = add_dpp<0x140>(v[r]);    // row_mirror
@@ -562,9 +564,11 @@ int residual_launch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
 template <typename TX, typename TY, bool BACK>
 int residual_dispatch(const ResidualArgs& a, unsigned grid, hipStream_t stream) {
   constexpr bool HALVES = sizeof(TY) == 2;
-  constexpr int N = HALVES ? 2 : 1;      // the three narrowest variants
+  constexpr int N = HALVES ? 2 : 1;      // the five narrowest variants
   const ResidualShape s = residual_shape(a.width, HALVES);
   switch (s.lanes * 100 + s.elems) {
+    case 400 / N + 4 * N: return residual_launch<TX, TY, BACK, 4 / N, 4 * N>(a, grid, stream);
+    case 800 / N + 4 * N: return residual_launch<TX, TY, BACK, 8 / N, 4 * N>(a, grid, stream);
     case 1600 / N + 4 * N: return residual_launch<TX, TY, BACK, 16 / N, 4 * N>(a, grid, stream);
     case 3200 / N + 4 * N: return residual_launch<TX, TY, BACK, 32 / N, 4 * N>(a, grid, stream);
     case 6400 / N + 4 * N: return residual_launch<TX, TY, BACK, 64 / N, 4 * N>(a, grid, stream);

@@ -97,7 +97,7 @@ static int pair_of(int stream_type, int block_type) {
 }
 
 static int check_desc(const disco_residual_norm* d) {
-  if (!d || d->rows < 0 || d->width < 1 || !(d->eps > 0.0f) || !isfinite(d->eps)) return DISCO_EINVAL;
+  if (!d || d->rows < 0 || d->width < 1 || !(d->eps > 0.0f) || !isfinite(d->eps) || !isfinite(d->scale)) return DISCO_EINVAL;
   if (d->param_type < DISCO_F32 || d->param_type > DISCO_BF16 || pair_of(d->stream_type, d->block_type) < 0) return DISCO_EINVAL;
   if (d->post_norm < DISCO_NORM_NONE || d->post_norm > DISCO_NORM_LAYER || d->pre_norm < DISCO_NORM_NONE || d->pre_norm > DISCO_NORM_LAYER)
     return DISCO_EINVAL;
@@ -201,7 +201,7 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
   a.partials = (g->dpost_weight || branch ? 1 : 0) | (g->dpost_bias || (branch && d->post_bias) ? 2 : 0) | (g->dpre_weight ? 4 : 0) |
                (g->dpre_bias ? 8 : 0);
   if (n > 0) {
-    if (!strided(g->ld_dx, n, F) || !strided(g->ld_dy, n, F) || (d->gate_kind == DISCO_GATE_FULL && g->dgate && !strided(g->ld_dgate, n, F)) ||
+    if ((g->dx && !strided(g->ld_dx, n, F)) || (g->dy && !strided(g->ld_dy, n, F)) || (d->gate_kind == DISCO_GATE_FULL && g->dgate && !strided(g->ld_dgate, n, F)) ||
         (d->gate_kind == DISCO_GATE_ROW && g->dgate && g->ld_dgate < 1 && n > 1))
       return DISCO_EINVAL;
     if (d->ldx < 0 || d->ldy < 0 || d->ld_gate < 0 || g->ld_dout < 0 || g->ld_dh < 0) return DISCO_EINVAL;
@@ -216,7 +216,7 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
   a.dout = g->dout; a.lddo = g->ld_dout; a.dh = g->dh; a.lddh = g->ld_dh;
   a.dx = g->dx; a.lddx = g->ld_dx; a.dy = g->dy; a.lddy = g->ld_dy; a.dg = channel ? nullptr : g->dgate; a.lddg = g->ld_dgate;
   a.partial = a.partials ? static_cast<float*>(workspace) : nullptr;
-  if (n > 0) {
+  if (n > 0 && (a.dx || a.dy || a.dg || a.partials)) {
     int r;
     switch (pair_of(d->stream_type, d->block_type)) {
       case kPairF32: r = residual_backward<kPairF32>(a, grid, stream); break;

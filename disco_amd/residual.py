@@ -9,7 +9,6 @@ networks need them.  There is no CPU fallback.
 """
 from __future__ import annotations
 
-import math
 from typing import Optional, Tuple, Union
 
 import torch
@@ -22,6 +21,7 @@ _ACTS = {None: 0, "sigmoid": 1, "tanh": 2}
 _NO_GATE, _FULL, _ROW, _CHANNEL = 0, 1, 2, 3
 _DTYPES = _lib.DTYPES
 _F32 = torch.float32
+_LEAST, _MOST = torch.finfo(_F32).tiny, torch.finfo(_F32).max
 
 
 class _Plan:
@@ -149,8 +149,8 @@ def _plan(x, block_dtype, post, pre, gate_kind, gate_act, scale, eps, has_block,
         raise ValueError(f"a norm is 'rms', 'layer' or None, got {post!r} and {pre!r}")
     if gate_act not in _ACTS:
         raise ValueError(f"gate_act is 'sigmoid', 'tanh' or None, got {gate_act!r}")
-    if not 0.0 < eps < math.inf:
-        raise ValueError(f"eps must be positive, got {eps}")
+    if not _LEAST <= eps <= _MOST:
+        raise ValueError(f"eps must be positive and finite in float32, got {eps}")
     dtype = None
     for name, v in vectors:
         if v is None:
@@ -252,8 +252,8 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: Optional[torch.Tens
         raise ValueError("gate_act needs a gate")
     if isinstance(scale, torch.Tensor):
         scale, vector = 1.0, scale
-    elif not -math.inf < scale < math.inf:
-        raise ValueError(f"scale must be finite, got {scale}")
+    elif not -_MOST <= scale <= _MOST:
+        raise ValueError(f"scale must be finite in float32, got {scale}")
     if post is None and (post_weight is not None or post_bias is not None):
         raise ValueError("post_weight and post_bias need a post norm")
     if pre is None and (pre_weight is not None or pre_bias is not None):

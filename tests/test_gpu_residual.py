@@ -153,7 +153,7 @@ def check(s, use=("out", "h"), what=""):
     return grads
 
 
-WIDTHS = [1, 2, 3, 4, 5, 41, 63, 64, 65, 100, 128, 129, 256, 257, 512, 513, 602, 768, 769, 1024, 1025, 1433, 2048, 2049, 4096, 4097, 8192,
+WIDTHS = [1, 2, 3, 4, 5, 7, 8, 15, 16, 17, 31, 32, 33, 41, 63, 64, 65, 100, 128, 129, 256, 257, 512, 513, 602, 768, 769, 1024, 1025, 1433, 2048, 2049, 4096, 4097, 8192,
           8193, 16383, 16384]
 
 
@@ -300,6 +300,18 @@ def test_broadcast_operands():
     assert abs(float(ga) - float(ref.sum())) <= C * float(ref.abs().sum())
 
 
+def test_a_gradient_with_one_repeated_row():
+    """Without a pre norm the stream's gradient is the given one, which may be a single row for all (stride 0)."""
+    for gate in (None, "row", "full"):
+        s = make(21, 40, pre=None, gate=gate, act="tanh", seed=44)
+        s["dout"] = torch.randn(1, 40, device=DEV).expand(21, 40)
+        check(s, ("out",))
+    x, y = (torch.randn(9, 24, device=DEV, requires_grad=True) for _ in range(2))
+    ops.residual_norm(x, y, post="rms").sum().backward()
+    assert torch.equal(x.grad, torch.ones_like(x))
+    ops.residual_norm(x.detach().requires_grad_(), y.detach()).sum().backward()      # nothing to compute
+
+
 def test_mixed_parameter_types_meet_in_float32():
     s = make(11, 40, "f32", "bf16", "f32", seed=43)
     s["t"]["post_weight"], s["t"]["pre_bias"] = s["t"]["post_weight"].bfloat16(), s["t"]["pre_bias"].half()
@@ -421,6 +433,20 @@ def test_many_rows_pass_32_bit_offsets():
     want = x[-3:].double() * torch.rsqrt(x[-3:].double().square().mean(1, keepdim=True) + EPS)
     assert ((h[-3:].double() - want).abs() <= 2.0 ** -11 * want.abs() * (1 + C) + C * want.abs() + 2.0 ** -24).all()
     assert not h[:1000].any() and not h[n // 2:n // 2 + 1000].any()
+    del h
+    x.requires_grad_()
+    w = torch.ones(F, device=DEV, requires_grad=True)
+    h = ops.row_norm(x, w, kind="rms", eps=EPS)
+    g = torch.zeros(n, F, dtype=torch.float16, device=DEV)
+    g[-2:] = 1.0
+    dx, dw = torch.autograd.grad(h, (x, w), g)
+    v = x.detach()[-2:].double().requires_grad_()
+    u = v * torch.rsqrt(v.square().mean(1, keepdim=True) + EPS)
+    (ref,) = torch.autograd.grad(u.sum(), v)
+    size = torch.rsqrt(v.detach().square().mean(1, keepdim=True) + EPS)
+    assert ((dx[-2:].double() - ref).abs() <= 2.0 ** -11 * ref.abs() * (1 + C) + C * F * size + 2.0 ** -24).all()
+    assert not dx[:1000].any() and not dx[-1000:-2].any()
+    assert ((dw.double() - u.detach().sum(0)).abs() <= C * u.detach().abs().sum(0)).all()
 
 
 @pytest.mark.parametrize("case", range(40))

@@ -20,7 +20,7 @@ def _xy(dtype=torch.float32, block=None):
     (dict(gate_act="sigmoid"), ValueError), (dict(gate=torch.zeros(N)), ValueError), (dict(gate=torch.zeros(N, 2)), ValueError),
     (dict(gate=torch.zeros(1, F)), ValueError), (dict(gate=torch.zeros(N, F, dtype=torch.float16)), TypeError),
     (dict(gate=torch.zeros(N, 1, dtype=torch.bfloat16)), TypeError), (dict(gate=torch.zeros(F, dtype=torch.float64)), TypeError),
-    (dict(scale=math.nan), ValueError), (dict(scale=math.inf), ValueError), (dict(scale=torch.zeros(F + 1)), ValueError),
+    (dict(scale=math.nan), ValueError), (dict(scale=math.inf), ValueError), (dict(scale=1e39), ValueError), (dict(eps=1e-46), ValueError), (dict(scale=torch.zeros(F + 1)), ValueError),
     (dict(scale=torch.zeros(())), ValueError), (dict(scale=torch.zeros(F, dtype=torch.int64)), TypeError),
     (dict(post_weight=torch.ones(F)), ValueError), (dict(post_bias=torch.ones(F)), ValueError),
     (dict(pre_weight=torch.ones(F)), ValueError), (dict(pre_bias=torch.ones(F)), ValueError),
@@ -87,7 +87,7 @@ def _desc(**k):
 
 @pytest.mark.parametrize("change", [
     dict(rows=-1), dict(width=0), dict(width=-3), dict(eps=0.0), dict(eps=-1.0), dict(eps=math.nan), dict(eps=math.inf),
-    dict(stream_type=3), dict(block_type=3), dict(stream_type=1), dict(stream_type=1, block_type=2), dict(param_type=-1),
+    dict(scale=math.nan), dict(scale=math.inf), dict(stream_type=3), dict(block_type=3), dict(stream_type=1), dict(stream_type=1, block_type=2), dict(param_type=-1),
     dict(post_norm=3), dict(pre_norm=-1), dict(gate_kind=4), dict(gate_act=3), dict(x=None), dict(y=None), dict(gate_kind=1),
     dict(gate_kind=2), dict(gate_kind=3), dict(post_weight=64), dict(pre_bias=64), dict(ldx=-1), dict(ldy=-8),
     dict(has_block=0), dict(has_block=0, pre_norm=1, post_norm=1), dict(has_block=0, pre_norm=1, scale_vector=64),
