@@ -132,9 +132,9 @@ static unsigned groups(int64_t rows, int threads, int lanes, int64_t most) {
 // norms, with half the bytes a wave, need 16: 179 us with 8, 141 with 16, 150 with 32.  Rows that several waves share
 // wait for each other, and want more (half rows of 5000: 383 us with 8, 304 with 16); so do gates for each element, whose
 // arithmetic shows (169343 x 256: 180 us with 8, 157 with 12).
-static unsigned forward_grid(int64_t rows, const ResidualShape& s, int mode, bool wide_stream, bool halves) {
+static unsigned forward_grid(int64_t rows, int64_t width, const ResidualShape& s, int mode, bool wide_stream, bool halves) {
   const int threads = residual_threads(s.lanes), y = halves ? 2 : 4, x = wide_stream ? 4 : 2;
-  const int bytes = 64 * s.elems * (x + (mode == kNormOnly ? 0 : mode == kJoin ? y : 2 * y));
+  const int bytes = (int)(64 * width / s.lanes) * (x + (mode == kNormOnly ? 0 : mode == kJoin ? y : 2 * y));
     const int fetched = (mode == kJoinGated ? 2 : 1) * (s.lanes <= 64 ? 16384 : s.lanes <= 256 ? 24576 : 32768);
   const int waves = std::max(8, std::min(32, (fetched + bytes - 1) / bytes));
   return groups(rows, threads, s.lanes, 256 * std::max(1, (waves * 64 + threads - 1) / threads));
@@ -165,7 +165,7 @@ extern "C" int disco_residual_norm_forward(const disco_residual_norm* d, void* o
   fill(d, &a);
   a.out = out; a.ldo = ld_out; a.h = h; a.ldh = ld_h; a.stats = stats;
   const ResidualShape s = residual_shape(F, d->block_type != DISCO_F32);
-  const unsigned grid = forward_grid(n, s, residual_mode(d->has_block, d->gate_kind), d->stream_type == DISCO_F32, d->block_type != DISCO_F32);
+  const unsigned grid = forward_grid(n, F, s, residual_mode(d->has_block, d->gate_kind), d->stream_type == DISCO_F32, d->block_type != DISCO_F32);
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   switch (pair_of(d->stream_type, d->block_type)) {
     case kPairF32: return residual_forward<kPairF32>(a, grid, stream);
