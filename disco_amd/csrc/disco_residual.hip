@@ -128,17 +128,18 @@ static unsigned groups(int64_t rows, int threads, int lanes, int64_t most) {
 }
 // The forward's waves: as many as keep FETCHED bytes of rows on their way to a compute unit (HBM answers after about a
 // microsecond at 20 GB/s for each), and no more: each further wave is one more place that memory is read and written at.
-// Joins of 200 M values, float32 rows of 256: 287 us with 8 waves, 308 with 16, 343 with 32; half rows of 256: 297, 322, 351;
-// norms, with half the bytes a wave, need 16: 179 us with 8, 141 with 16, 150 with 32.  Rows that several waves share
+// Joins of 100 M float32 or 200 M half values, float32 rows of 256: 287 us with 8 waves, 308 with 16, 343 with 32; half rows:
+// 297, 322, 351; norms, with half the bytes a wave, need 16: 179 us with 8, 141 with 16, 150 with 32.  Rows that several waves share
 // wait for each other, and want more (half rows of 5000: 383 us with 8, 304 with 16); so do gates for each element, whose
 // arithmetic shows (169343 x 256: 180 us with 8, 157 with 12).
 static unsigned forward_grid(int64_t rows, int64_t width, const ResidualShape& s, int mode, bool wide_stream, bool halves) {
   const int threads = residual_threads(s.lanes), y = halves ? 2 : 4, x = wide_stream ? 4 : 2;
   const int bytes = (int)(64 * width / s.lanes) * (x + (mode == kNormOnly ? 0 : mode == kJoin ? y : 2 * y));
-    const int fetched = (mode == kJoinGated ? 2 : 1) * (s.lanes <= 64 ? 16384 : s.lanes <= 256 ? 24576 : 32768);
+  const int fetched = (mode == kJoinGated ? 2 : 1) * (s.lanes <= 64 ? 16384 : s.lanes <= 256 ? 24576 : 32768);
   const int waves = std::max(8, std::min(32, (fetched + bytes - 1) / bytes));
   return groups(rows, threads, s.lanes, 256 * std::max(1, (waves * 64 + threads - 1) / threads));
 }
+
 // The backward's number is also the number of partial sums that the finish reads again.
 static unsigned backward_grid(int64_t rows, const ResidualShape& s, int mode) {
   const int threads = residual_back_threads(s.lanes, s.elems, mode);

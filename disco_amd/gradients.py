@@ -23,13 +23,17 @@ def _tensors(grads) -> List[torch.Tensor]:
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     if not grads:
         return grads
-    if not all([isinstance(g, torch.Tensor) and g.layout is torch.strided for g in grads]):
+    if not all([isinstance(g, torch.Tensor) for g in grads]):
         raise TypeError("gradients must be dense tensors")
-    if not {g.dtype for g in grads} <= _lib.DTYPES.keys():
-        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {sorted({str(g.dtype) for g in grads})}")
-    device = grads[0].device
-    if any([g.device != device for g in grads]):
-        raise ValueError(f"gradients on {sorted({str(g.device) for g in grads})}: one device at a time")
+    kinds = {(g.layout, g.dtype, g.device) for g in grads}
+    if len(kinds) == 1 and grads[0].layout is torch.strided and grads[0].dtype in _lib.DTYPES:
+        return grads
+    if any([layout is not torch.strided for layout, _, _ in kinds]):
+        raise TypeError("gradients must be dense tensors")
+    if not {dtype for _, dtype, _ in kinds} <= _lib.DTYPES.keys():
+        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {sorted({str(dtype) for _, dtype, _ in kinds})}")
+    if len({device for _, _, device in kinds}) > 1:
+        raise ValueError(f"gradients on {sorted({str(device) for _, _, device in kinds})}: one device at a time")
     return grads
 
 
@@ -45,6 +49,11 @@ def _norm_type(norm_type) -> int:
     return p
 
 
+def _codes(tensors) -> array:
+    codes = _lib.DTYPES
+    return array("i", [codes[t.dtype] for t in tensors])
+
+
 def _launch(grads: Sequence[torch.Tensor], p: int, max_norm: Optional[float], out) -> torch.Tensor:
     first = grads[0]
     index = first.get_device()
@@ -53,10 +62,9 @@ def _launch(grads: Sequence[torch.Tensor], p: int, max_norm: Optional[float], ou
             return _launch(grads, p, max_norm, out)
     lib = _lib.load()
     n = len(grads)
-    codes = _lib.DTYPES
     src = array("Q", [g.data_ptr() for g in grads])
     numel = array("q", [g.numel() for g in grads])
-    types = array("i", [codes[g.dtype] for g in grads])
+    types = _codes(grads)
     nb = lib.disco_grad_norm_workspace_bytes(n)
     ws = torch.empty(nb, dtype=torch.uint8, device=first.device)
     norm = torch.empty((), dtype=torch.float32, device=first.device)
@@ -68,14 +76,17 @@ def _launch(grads: Sequence[torch.Tensor], p: int, max_norm: Optional[float], ou
     else:
         same = out is grads
         dst = src if same else array("Q", [o.data_ptr() for o in out])
-        to = types if same else array("i", [codes[o.dtype] for o in out])
+        to = types if same else _codes(out)
         status = lib.disco_grad_clip(src.buffer_info()[0], dst.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0],
                                      to.buffer_info()[0], n, p, max_norm, norm.data_ptr(), ws.data_ptr(), nb, stream)
         if status == -1:
             raise ValueError(_SHARED)
         _lib.check(status, "disco_grad_clip")
         # written behind autograd's back: whoever saved one of them must notice
-        torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
+        try:
+            torch.autograd.graph.increment_version(out)
+        except RuntimeError:      # tensors made in inference mode keep no version
+            torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
     return norm
 
 
@@ -121,10 +132,11 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         dst = _tensors(out)
         if len(dst) != len(grads):
             raise ValueError(f"out has {len(dst)} tensors for {len(grads)} gradients")
+        f32 = torch.float32
         if dst and dst[0].device != grads[0].device or any(
-                [o.shape != g.shape or (o.dtype != torch.float32 and o.dtype != g.dtype) for g, o in zip(grads, dst)]):
+                [o.shape != g.shape or (o.dtype is not f32 and o.dtype is not g.dtype) for g, o in zip(grads, dst)]):
             for g, o in zip(grads, dst):
-                if o.shape == g.shape and o.device == g.device and o.dtype in (g.dtype, torch.float32):
+                if o.shape == g.shape and o.device == g.device and o.dtype in (g.dtype, f32):
                     continue
                 raise ValueError(f"out must have the gradients' shapes and device and their type or float32, got {tuple(o.shape)} "
                                  f"{o.dtype} on {o.device} for {tuple(g.shape)} {g.dtype} on {g.device}")

@@ -235,3 +235,18 @@ def test_drawn_cases(case):
     to = [torch.empty_like(g, dtype=[g.dtype, torch.float32][int(r.integers(2))]) for g in grads]
     check_norm(ops.clip_grads(grads, want * 0.5, p, out=to), want)
     check_clip(grads, to, want * 0.5, want)
+
+
+def test_clipping_is_seen_by_autograd():
+    """Gradients written in place count as modified: a graph that saved one of them refuses to use it."""
+    x = torch.randn(50, device=DEV, requires_grad=True)
+    g = torch.randn(50, device=DEV)
+    y = x * g
+    ops.clip_grads([g], 1e-3)
+    with pytest.raises(RuntimeError, match="modified"):
+        y.sum().backward()
+    with torch.inference_mode():
+        h = torch.ones(10, device=DEV)
+        check_norm(ops.clip_grads([h], 1.0), math.sqrt(10.0))
+    want = norm64([h], 2)                        # max_norm * norm / (norm + 1e-6), not quite max_norm
+    check_norm(ops.clip_grads([h, torch.zeros(3, device=DEV)], 5.0), want)
