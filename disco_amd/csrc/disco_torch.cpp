@@ -1,0 +1,183 @@
+// disco_torch.cpp -- the residual join as an autograd node of its own (host code; the kernels are libdisco_hip.so's).
+//
+// A training pass over few rows is bound by what the host does around two launches: with the node in Python, whose backward
+// has to take the interpreter from the thread that waits for it, a pass of forward and eight gradients took 213 us of host
+// time, and takes 116 here (the forward 46 and 17).  Arguments are checked in disco_amd/residual.py; this file allocates, calls the C entries and keeps what the
+// backward reads.  The entries' addresses come from the loaded library (bind), so there is one copy of it in the process.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <cstdint>
+#include <memory>
+#include <optional>
+#include <vector>
+
+#include "../../include/disco_hip.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+decltype(&disco_residual_norm_forward) g_forward = nullptr;
+decltype(&disco_residual_norm_backward) g_backward = nullptr;
+decltype(&disco_residual_norm_workspace_bytes) g_workspace = nullptr;
+decltype(&disco_status_string) g_status = nullptr;
+
+void bind(int64_t forward, int64_t backward, int64_t workspace, int64_t status) {
+  g_forward = reinterpret_cast<decltype(g_forward)>(forward);
+  g_backward = reinterpret_cast<decltype(g_backward)>(backward);
+  g_workspace = reinterpret_cast<decltype(g_workspace)>(workspace);
+  g_status = reinterpret_cast<decltype(g_status)>(status);
+}
+
+void check(int status, const char* what) { TORCH_CHECK(status == DISCO_OK, what, ": ", g_status(status)); }
+
+// What a call does besides its tensors, as residual.py packs it: two bits each of the post norm, the pre norm, the gate, its
+// activation, the block's and the parameters' type, and one for the block itself.
+struct Plan {
+  int post, pre, gate, act, block_type, param_type, block;
+  explicit Plan(int64_t p)
+      : post(p & 3), pre(p >> 2 & 3), gate(p >> 4 & 3), act(p >> 6 & 3), block_type(p >> 8 & 3), param_type(p >> 10 & 3), block(p >> 12 & 1) {}
+};
+
+int type_code(const Tensor& t) {
+  const auto s = t.scalar_type();
+  return s == at::kFloat ? DISCO_F32 : s == at::kHalf ? DISCO_F16 : DISCO_BF16;
+}
+at::ScalarType type_of(int code) { return code == DISCO_F32 ? at::kFloat : code == DISCO_F16 ? at::kHalf : at::kBFloat16; }
+const void* read(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void* write(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+int64_t pitch(const Tensor& t, int64_t width) { return t.defined() ? t.stride(0) : width; }
+
+// x, y, gate, scale, post weight and bias, pre weight and bias; an absent one is undefined
+struct Operands { Tensor x, y, gate, scale, w1, b1, w2, b2; };
+using Maybe = std::optional<Tensor>;
+Operands operands(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1, const Maybe& w2,
+                  const Maybe& b2) {
+  const auto get = [](const Maybe& t) { return t.has_value() ? *t : Tensor(); };
+  return {x, get(y), get(gate), get(scale), get(w1), get(b1), get(w2), get(b2)};
+}
+
+disco_residual_norm describe(const Plan& p, const Operands& o, double scale, double eps) {
+  disco_residual_norm d{};
+  d.rows = o.x.size(0); d.width = o.x.size(1);
+  d.ldx = o.x.stride(0); d.ldy = o.y.defined() ? o.y.stride(0) : 0; d.ld_gate = o.gate.defined() ? o.gate.stride(0) : 0;
+  d.x = read(o.x); d.y = read(o.y); d.gate = read(o.gate);
+  d.post_weight = read(o.w1); d.post_bias = read(o.b1); d.pre_weight = read(o.w2); d.pre_bias = read(o.b2); d.scale_vector = read(o.scale);
+  d.stream_type = type_code(o.x); d.block_type = p.block_type; d.param_type = p.param_type;
+  d.has_block = p.block; d.post_norm = p.post; d.pre_norm = p.pre; d.gate_kind = p.gate; d.gate_act = p.act;
+  d.scale = (float)scale; d.eps = (float)eps;
+  return d;
+}
+
+struct Outputs { Tensor out, h, stats; };
+
+// Output rows lie densely: columns that nothing writes between them leave cache lines half written (the norm of 2.4 M rows of
+// 41 floats: 268 us with rows padded to 44, 170 dense).
+Outputs forward(const Plan& p, const Operands& o, double scale, double eps, int64_t stream, bool keep) {
+  const c10::DeviceGuard guard(o.x.device());
+  Outputs r;
+  if (p.block) r.out = at::empty(o.x.sizes(), o.x.options());
+  if (p.pre) r.h = at::empty(o.x.sizes(), o.x.options().dtype(type_of(p.block_type)));
+  if (keep) r.stats = at::empty({4 * o.x.size(0)}, o.x.options().dtype(at::kFloat));
+  const disco_residual_norm d = describe(p, o, scale, eps);
+  check(g_forward(&d, write(r.out), pitch(r.out, 0), write(r.h), pitch(r.h, 0), static_cast<float*>(write(r.stats)), reinterpret_cast<void*>(stream)),
+        "disco_residual_norm_forward");
+  return r;
+}
+
+// Rows with unit column stride that do not overlap, or one row for all: the tensor or a copy.
+Tensor rows(const Tensor& t) {
+  if (!t.defined() || t.is_contiguous()) return t;
+  const int64_t n = t.size(0), width = t.size(1), r = t.stride(0), c = t.stride(1);
+  return (width > 1 && c != 1) || (n > 1 && r > 0 && r < width) ? t.contiguous() : t;
+}
+
+class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
+ public:
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1,
+                               const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t stream) {
+    const Plan p(plan);
+    const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
+    Outputs r = ::forward(p, o, factor, eps, stream, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({o.x, o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, r.stats});
+    // the node runs on its forward's stream, whichever one its caller is on
+    ctx->saved_data["ints"] = std::vector<int64_t>{plan, stream};
+    ctx->saved_data["floats"] = std::vector<double>{factor, eps};
+    variable_list outputs;
+    if (p.block) outputs.push_back(r.out);
+    if (p.pre) outputs.push_back(r.h);
+    return outputs;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list result(12);
+    const auto ints = ctx->saved_data["ints"].toIntVector();
+    const auto floats = ctx->saved_data["floats"].toDoubleVector();
+    const Plan p(ints[0]);
+    const Tensor dout = p.block ? rows(grads[0]) : Tensor(), dh = p.pre ? rows(grads[p.block ? 1 : 0]) : Tensor();
+    if (!dout.defined() && !dh.defined()) return result;
+    const variable_list s = ctx->get_saved_variables();
+    const Operands o{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
+    const c10::DeviceGuard guard(o.x.device());
+    const int64_t n = o.x.size(0), width = o.x.size(1);
+    // without a gradient of h the stream's gradient is that of out itself
+    const bool through = !dh.defined();
+    for (size_t i = 0, edge = 0; i < 8; ++i) {      // edges are numbered over the operands that are there
+      if (!s[i].defined() || !ctx->needs_input_grad(edge++)) continue;
+      if (through && (i == 0 || i >= 6)) continue;
+      result[i] = at::empty(s[i].sizes(), s[i].options());
+    }
+    const size_t bytes = g_workspace(n, width);
+    const Tensor ws = at::empty({(int64_t)bytes}, o.x.options().dtype(at::kByte));
+    const disco_residual_norm d = describe(p, o, floats[0], floats[1]);
+    disco_residual_norm_grads g{};
+    g.dout = read(dout); g.dh = read(dh);
+    g.dx = write(result[0]); g.dy = write(result[1]); g.dgate = write(result[2]); g.dscale = write(result[3]);
+    g.dpost_weight = write(result[4]); g.dpost_bias = write(result[5]); g.dpre_weight = write(result[6]); g.dpre_bias = write(result[7]);
+    g.ld_dout = pitch(dout, width); g.ld_dh = pitch(dh, width); g.ld_dx = pitch(result[0], width); g.ld_dy = pitch(result[1], width);
+    g.ld_dgate = pitch(result[2], width);
+    check(g_backward(&d, static_cast<const float*>(read(s[8])), &g, write(ws), bytes, reinterpret_cast<void*>(ints[1])), "disco_residual_norm_backward");
+    if (through && ctx->needs_input_grad(0)) result[0] = dout;
+    if (at::GradMode::is_enabled()) {      // the gradients have no formula of their own: whoever differentiates them is told
+      for (Tensor& t : result)
+        if (t.defined()) t = t.detach().requires_grad_();
+      const auto refuse = std::make_shared<torch::autograd::DelayedError>("residual_norm has no second derivatives", 12);
+      return (*refuse)(std::move(result));
+    }
+    return result;
+  }
+};
+
+std::vector<Tensor> residual_norm(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1,
+                                  const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t stream) {
+  TORCH_CHECK(g_forward && g_backward && g_workspace && g_status, "disco_torch: not bound to libdisco_hip.so");
+  TORCH_CHECK(x.is_cuda(), "x is on ", x.device(), ": disco_amd runs on the GPU only, there is no CPU fallback");
+  const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
+  bool grad = false;
+  if (at::GradMode::is_enabled())
+    for (const Tensor* t : {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2}) grad = grad || (t->defined() && t->requires_grad());
+  if (grad) return ResidualNorm::apply(x, y, gate, scale, w1, b1, w2, b2, plan, factor, eps, stream);
+  const Plan p(plan);
+  const Outputs r = forward(p, o, factor, eps, stream, false);
+  std::vector<Tensor> outputs;
+  if (p.block) outputs.push_back(r.out);
+  if (p.pre) outputs.push_back(r.h);
+  return outputs;
+}
+
+}  // namespace
+
+TORCH_LIBRARY(disco_amd, m) {
+  m.def("bind(int forward, int backward, int workspace, int status) -> ()", &bind);
+  m.def(
+      "residual_norm(Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? post_weight, Tensor? post_bias, Tensor? pre_weight, "
+      "Tensor? pre_bias, int plan, float factor, float eps, int stream) -> Tensor[]",
+      &residual_norm);
+}

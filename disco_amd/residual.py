@@ -5,15 +5,13 @@
 
 and the norm before the first block (``row_norm``).  Both are differentiable in every tensor.  The reference normalises
 hidden layers with stock BatchNorm (/root/reference/models/basicgnn_large.py:119-133) and has no residual blocks; deep
-networks need them.  There is no CPU fallback.
+networks need them.  The arguments are checked here; the autograd node is disco_torch.cpp's.  There is no CPU fallback.
 """
 from __future__ import annotations
 
 from typing import Optional, Tuple, Union
 
 import torch
-from torch.autograd.function import once_differentiable
-
 from . import _lib
 
 _KINDS = {None: 0, "rms": 1, "layer": 2}
@@ -22,11 +20,6 @@ _NO_GATE, _FULL, _ROW, _CHANNEL = 0, 1, 2, 3
 _DTYPES = _lib.DTYPES
 _F32 = torch.float32
 _LEAST, _MOST = torch.finfo(_F32).tiny, torch.finfo(_F32).max
-
-
-class _Plan:
-    """What a call does besides its tensors."""
-    __slots__ = ("post", "pre", "gate", "act", "scale", "eps", "block_dtype", "param_dtype", "has_block", "index")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -40,89 +33,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _ptr(t):
-    return 0 if t is None else t.data_ptr()
-
-
-def _describe(plan, x, y, gate, scale, w1, b1, w2, b2) -> "_lib.ResidualNorm":
-    n, F = x.shape
-    return _lib.ResidualNorm(
-        n, F, x.stride(0), 0 if y is None else y.stride(0), 0 if gate is None else gate.stride(0), x.data_ptr(), _ptr(y), _ptr(gate),
-        _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(scale), _DTYPES[x.dtype], _DTYPES[plan.block_dtype], _DTYPES[plan.param_dtype],
-        plan.has_block, plan.post, plan.pre, plan.gate, plan.act, plan.scale, plan.eps)
-
-
-def _forward(plan, x, y, gate, scale, w1, b1, w2, b2, keep: bool):
-    if plan.index != torch.cuda.current_device():
-        with torch.cuda.device(plan.index):
-            return _forward(plan, x, y, gate, scale, w1, b1, w2, b2, keep)
-    # dense rows: columns that nothing writes between them leave cache lines half written (the norm of 2.4 M rows of 41 floats:
-    # 268 us with rows padded to 44, 170 dense)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device) if plan.has_block else None
-    h = torch.empty(x.shape, dtype=plan.block_dtype, device=x.device) if plan.pre else None
-    stats = torch.empty(4 * x.shape[0], dtype=_F32, device=x.device) if keep else None
-    status = _lib.load().disco_residual_norm_forward(
-        _describe(plan, x, y, gate, scale, w1, b1, w2, b2), _ptr(out), 0 if out is None else out.stride(0), _ptr(h),
-        0 if h is None else h.stride(0), _ptr(stats), _lib.stream_of(plan.index))
-    if status:
-        _lib.check(status, "disco_residual_norm_forward")
-    return out, h, stats
-
-
-def _backward(plan, needs, dout, dh, x, y, gate, scale, w1, b1, w2, b2, stats):
-    if plan.index != torch.cuda.current_device():
-        with torch.cuda.device(plan.index):
-            return _backward(plan, needs, dout, dh, x, y, gate, scale, w1, b1, w2, b2, stats)
-    n, F = x.shape
-    dout = None if dout is None else _rows(dout)
-    dh = None if dh is None else _rows(dh)
-
-    def like(t, wanted):
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
-
-    nx, ny, ng, ns, nw1, nb1, nw2, nb2 = needs
-    # without a gradient of h the stream's gradient is that of out itself
-    through = dh is None
-    dx = (dout if nx else None) if through else like(x, nx)
-    dy, dg, ds, dw1, db1 = like(y, ny), like(gate, ng), like(scale, ns), like(w1, nw1), like(b1, nb1)
-    dw2, db2 = (None, None) if through else (like(w2, nw2), like(b2, nb2))
-    lib = _lib.load()
-    nb = lib.disco_residual_norm_workspace_bytes(n, F)
-    ws = torch.empty(nb, dtype=torch.uint8, device=x.device)
-
-    def stride(t):
-        return F if t is None else t.stride(0)
-
-    g = _lib.ResidualNormGrads(_ptr(dout), _ptr(dh), 0 if through else _ptr(dx), _ptr(dy), _ptr(dg), stride(dout), stride(dh), stride(dx),
-                               stride(dy), stride(dg), _ptr(dw1), _ptr(db1), _ptr(dw2), _ptr(db2), _ptr(ds))
-    status = lib.disco_residual_norm_backward(_describe(plan, x, y, gate, scale, w1, b1, w2, b2), _ptr(stats), g, ws.data_ptr(), nb,
-                                              _lib.stream_of(plan.index))
-    if status:
-        _lib.check(status, "disco_residual_norm_backward")
-    return None, dx, dy, dg, ds, dw1, db1, dw2, db2
-
-
-class _ResidualNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, plan, x, y, gate, scale, w1, b1, w2, b2):
-        out, h, stats = _forward(plan, x, y, gate, scale, w1, b1, w2, b2, True)
-        ctx.plan = plan
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, y, gate, scale, w1, b1, w2, b2, stats)
-        if out is None:
-            return h
-        return out if h is None else (out, h)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        plan = ctx.plan
-        dout, dh = grads if len(grads) == 2 else (grads[0], None) if plan.has_block else (None, grads[0])
-        if dout is None and dh is None:
-            return (None,) * 9
-        return _backward(plan, ctx.needs_input_grad[1:], dout, dh, *ctx.saved_tensors)
-
-
 def _matrix(x, what: str):
     if not isinstance(x, torch.Tensor) or x.layout is not torch.strided:
         raise TypeError(f"{what} must be a dense tensor")
@@ -131,8 +41,9 @@ def _matrix(x, what: str):
     return x
 
 
-def _plan(x, block_dtype, post, pre, gate_kind, gate_act, scale, eps, has_block, vectors) -> _Plan:
-    """Checks what the tensors and options have to be, and settles the parameters' type: theirs, or float32 where they differ."""
+def _plan(x, block_dtype, post, pre, gate_kind, gate_act, eps, has_block, vectors):
+    """Checks what the tensors and options have to be.  Returns the call's options, packed as disco_torch.cpp reads them, and the
+    parameters' type: theirs, or float32 where they differ."""
     F, device = x.shape[1], x.device
     if not 1 <= F <= _lib.RESIDUAL_MAX_WIDTH:
         raise ValueError(f"width {F} is outside 1 .. {_lib.RESIDUAL_MAX_WIDTH}")
@@ -160,41 +71,29 @@ def _plan(x, block_dtype, post, pre, gate_kind, gate_act, scale, eps, has_block,
         dtype = v.dtype if dtype is None or dtype == v.dtype else _F32
     if not x.is_cuda:
         raise RuntimeError(f"x is on {device}: disco_amd runs on the GPU only, there is no CPU fallback")
-    plan = _Plan()
-    plan.post, plan.pre, plan.gate, plan.act = _KINDS[post], _KINDS[pre], gate_kind, _ACTS[gate_act]
-    plan.scale, plan.eps, plan.block_dtype, plan.has_block = scale, eps, block_dtype, has_block
-    plan.param_dtype, plan.index = dtype or _F32, x.get_device()
-    return plan
+    dtype = dtype or _F32
+    return (_KINDS[post] | _KINDS[pre] << 2 | gate_kind << 4 | _ACTS[gate_act] << 6 | _DTYPES[block_dtype] << 8 | _DTYPES[dtype] << 10
+            | has_block << 12), dtype
 
 
-def _run(plan, x, y, gate, vectors):
-    """The call itself: tensors as the kernels read them, through autograd where one of them needs a gradient."""
-    x = _rows(x)
-    if y is not None:
-        y = _rows(y)
-    if plan.gate == _FULL:
+def _vector(v, dtype):
+    if v is None:
+        return None
+    if v.dtype != dtype:
+        v = v.to(dtype)
+    return v if v.is_contiguous() else v.contiguous()
+
+
+def _run(plan, x, y, gate, scale, eps, vectors):
+    """The call itself, of tensors as the kernels read them; through autograd where one of them needs a gradient."""
+    options, dtype = plan
+    (_, channel), *rest = vectors
+    if channel is not None:
+        gate = _vector(channel, dtype)
+    elif gate is not None and gate.shape[1] > 1:
         gate = _rows(gate)
-    grads = torch.is_grad_enabled() and (x.requires_grad or (y is not None and y.requires_grad) or (gate is not None and gate.requires_grad))
-    dtype = plan.param_dtype
-    tensors = [x, y, gate]
-    for name, v in vectors:
-        if v is not None:
-            grads = grads or (v.requires_grad and torch.is_grad_enabled())
-            if v.dtype != dtype:
-                v = v.to(dtype)
-            if not v.is_contiguous():
-                v = v.contiguous()
-        if name == "gate":
-            if v is not None:
-                tensors[2] = v
-        else:
-            tensors.append(v)
-    if grads:
-        return _ResidualNormFn.apply(plan, *tensors)
-    out, h, _ = _forward(plan, *tensors, False)
-    if out is None:
-        return h
-    return out if h is None else (out, h)
+    return _lib.residual_op()(_rows(x), None if y is None else _rows(y), gate, *[_vector(v, dtype) for _, v in rest], options, scale, eps,
+                              _lib.stream_of(x.get_device()))
 
 
 def row_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, kind: str = "layer",
@@ -206,8 +105,8 @@ def row_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optio
     _matrix(x, "x")
     if kind is None:
         raise ValueError("kind is 'rms' or 'layer'")
-    vectors = (("scale", None), ("post_weight", None), ("post_bias", None), ("weight", weight), ("bias", bias))
-    return _run(_plan(x, dtype or x.dtype, None, kind, _NO_GATE, None, 1.0, eps, False, vectors), x, None, None, vectors)
+    vectors = (("gate", None), ("scale", None), ("post_weight", None), ("post_bias", None), ("weight", weight), ("bias", bias))
+    return _run(_plan(x, dtype or x.dtype, None, kind, _NO_GATE, None, eps, False, vectors), x, None, None, 1.0, eps, vectors)[0]
 
 
 def residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: Optional[torch.Tensor] = None, gate_act: Optional[str] = None,
@@ -254,4 +153,5 @@ def residual_norm(x: torch.Tensor, y: torch.Tensor, *, gate: Optional[torch.Tens
         raise ValueError("pre_weight and pre_bias need a pre norm")
     vectors = (("gate", channel), ("scale", vector), ("post_weight", post_weight), ("post_bias", post_bias), ("pre_weight", pre_weight),
                ("pre_bias", pre_bias))
-    return _run(_plan(x, y.dtype, post, pre, kind, gate_act, scale, eps, True, vectors), x, y, gate, vectors)
+    got = _run(_plan(x, y.dtype, post, pre, kind, gate_act, eps, True, vectors), x, y, gate, scale, eps, vectors)
+    return got[0] if pre is None else tuple(got)

@@ -415,11 +415,67 @@ def test_captured_training_step_replays():
             assert torch.equal(a, b), i
 
 
+def test_backward_from_another_stream_and_thread():
+    """A node runs on its forward's stream, whichever one its caller is on; calls from two threads do not disturb each other."""
+    import threading
+    s = make(3000, 120, seed=72)
+    want = train(s)
+    side = torch.cuda.Stream()
+    t = {k: v.clone().requires_grad_() for k, v in s["t"].items()}
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        out, h = call(s, t)
+    torch.cuda.current_stream().wait_stream(side)
+    for k, g in zip(t, torch.autograd.grad([out, h], list(t.values()), [s["dout"], s["dh"]])):
+        assert torch.equal(g, want[2][k]), k
+    got = [None] * 4
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+            for _ in range(5):
+                got[i] = train(s)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    [w.start() for w in threads]
+    [w.join() for w in threads]
+    for r in got:
+        assert torch.equal(r[0], want[0]) and torch.equal(r[1], want[1]) and all(torch.equal(r[2][k], want[2][k]) for k in want[2])
+
+
+def test_what_autograd_keeps():
+    """Operands changed in between are noticed, kept ones may move to the host and back, one tensor may be several operands."""
+    s = make(20, 30)
+    t = {k: v.clone().requires_grad_() for k, v in s["t"].items()}
+    z = t["y"] * 1.0
+    out, h = call(s, {**t, "y": z})
+    z.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        out.sum().backward()
+    want = train(s)
+    with torch.autograd.graph.save_on_cpu():
+        got = train(s)
+    assert all(torch.equal(got[2][k], want[2][k]) for k in want[2])
+    with torch.inference_mode():
+        out, h = call(s)
+    assert torch.equal(out, want[0]) and torch.equal(h, want[1])
+    x, w = torch.randn(9, 16, device=DEV, requires_grad=True), torch.randn(16, device=DEV, requires_grad=True)
+    out = ops.residual_norm(x, x, gate=x, post="rms", post_weight=w, scale=w)
+    gx, gw = torch.autograd.grad(out.sum(), (x, w))
+    X, W = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    u = X * torch.rsqrt((X * X).mean(1, keepdim=True) + EPS)
+    for a, b in zip((gx, gw), torch.autograd.grad((X + W * X * u * W).sum(), (X, W))):
+        assert ((a.double() - b).abs() <= C * (1 + b.abs().max())).all()
+
+
 def test_second_derivatives_are_refused():
     s = make(4, 16, gate=None, act=None)
     t = {k: v.clone().requires_grad_() for k, v in s["t"].items()}
     out, h = call(s, t)
     (g,) = torch.autograd.grad(out.sum() + h.square().sum(), t["x"], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        g.sum().backward(retain_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), t["x"])
 

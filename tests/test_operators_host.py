@@ -178,3 +178,10 @@ def test_residual_models_refuse_and_leave_the_others_alone():
         ResidualNorm(8)(torch.zeros(4, 8), torch.zeros(4, 8), torch.zeros(4, 8))
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         RowNorm(8)(torch.zeros(4, 8))
+
+
+def test_the_torch_operator_is_built_and_bound():
+    op = _lib.residual_op()
+    assert "libdisco_torch.so" in open("/proc/self/maps").read()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        op(torch.zeros(4, 8), None, None, None, None, None, None, None, 1 << 2, 1.0, 1e-5, 0)
