@@ -14,7 +14,7 @@ import torch  # (loads the process's HIP runtime before our library binds to it)
 from .build import lib_path
 
 _lib = None
-_residual_op = None
+_torch_ops = {}
 
 c_void_p, c_int, c_int64, c_size_t = C.c_void_p, C.c_int, C.c_int64, C.c_size_t
 
@@ -160,19 +160,21 @@ def load(path: str | None = None):
     return lib
 
 
-def residual_op():
-    """The residual join as a torch operator (libdisco_torch.so, disco_torch.cpp), bound to the loaded libdisco_hip.so."""
-    global _residual_op
-    if _residual_op is None:
+def torch_op(name: str):
+    """An operator of libdisco_torch.so (disco_torch.cpp), bound to the loaded libdisco_hip.so."""
+    op = _torch_ops.get(name)
+    if op is None:
         lib = load()
-        p = lib_path("libdisco_torch.so")
-        if not os.path.exists(p):
-            raise RuntimeError(f"{p} not found: run `python -m disco_amd.build` (or __graft_entry__.build())")
-        torch.ops.load_library(p)
-        torch.ops.disco_amd.bind(*[C.cast(getattr(lib, n), c_void_p).value for n in (
-            "disco_residual_norm_forward", "disco_residual_norm_backward", "disco_residual_norm_workspace_bytes", "disco_status_string")])
-        _residual_op = torch.ops.disco_amd.residual_norm.default
-    return _residual_op
+        if not _torch_ops:
+            p = lib_path("libdisco_torch.so")
+            if not os.path.exists(p):
+                raise RuntimeError(f"{p} not found: run `python -m disco_amd.build` (or __graft_entry__.build())")
+            torch.ops.load_library(p)
+            torch.ops.disco_amd.bind(*[C.cast(getattr(lib, n), c_void_p).value for n in (
+                "disco_residual_norm_forward", "disco_residual_norm_backward", "disco_residual_norm_workspace_bytes", "disco_status_string",
+                "disco_grad_norm", "disco_grad_clip", "disco_grad_norm_workspace_bytes")])
+        op = _torch_ops[name] = getattr(torch.ops.disco_amd, name).default
+    return op
 
 
 class DiscoError(RuntimeError):

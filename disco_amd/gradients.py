@@ -7,7 +7,6 @@ nothing synchronises.  No counterpart in the reference, whose training loops do 
 from __future__ import annotations
 
 import math
-from array import array
 from typing import Iterable, List, Optional, Sequence, Union
 
 import torch
@@ -18,27 +17,28 @@ _NORMS = {1.0: 1, 2.0: 2, math.inf: 0}
 _SHARED = "clip_grads: two tensors share memory; each gradient may be scaled only once"
 
 
-def _tensors(grads) -> List[torch.Tensor]:
-    """The list of gradients.  The checks go list by list rather than tensor by tensor: a model has hundreds of them."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    if not grads:
-        return grads
-    if not all([isinstance(g, torch.Tensor) for g in grads]):
+def _list(tensors) -> List[torch.Tensor]:
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    if not all([isinstance(t, torch.Tensor) for t in tensors]):
         raise TypeError("gradients must be dense tensors")
-    kinds = {(g.layout, g.dtype, g.device) for g in grads}
-    if len(kinds) == 1 and grads[0].layout is torch.strided and grads[0].dtype in _lib.DTYPES:
-        return grads
-    if any([layout is not torch.strided for layout, _, _ in kinds]):
-        raise TypeError("gradients must be dense tensors")
-    if not {dtype for _, dtype, _ in kinds} <= _lib.DTYPES.keys():
-        raise TypeError(f"gradients must be float32, float16 or bfloat16, got {sorted({str(dtype) for _, dtype, _ in kinds})}")
-    if len({device for _, _, device in kinds}) > 1:
-        raise ValueError(f"gradients on {sorted({str(device) for _, _, device in kinds})}: one device at a time")
-    return grads
+    return tensors
 
 
-def _on_gpu(grads) -> None:
-    if grads and not grads[0].is_cuda:
+def _check(grads, out=()) -> None:
+    """Says what is wrong with tensors that the kernels did not take, if it is not how they lie."""
+    for g in [*grads, *out]:
+        if g.layout is not torch.strided:
+            raise TypeError("gradients must be dense tensors")
+        if g.dtype not in _lib.DTYPES:
+            raise TypeError(f"gradients must be float32, float16 or bfloat16, got {g.dtype}")
+    for g, o in zip(grads, out):
+        if o.shape != g.shape or o.device != g.device or o.dtype not in (g.dtype, torch.float32):
+            raise ValueError(f"out must have the gradients' shapes and device and their type or float32, got {tuple(o.shape)} "
+                             f"{o.dtype} on {o.device} for {tuple(g.shape)} {g.dtype} on {g.device}")
+    for g in grads:
+        if g.device != grads[0].device:
+            raise ValueError(f"gradients on {grads[0].device} and {g.device}: one device at a time")
+    if not grads[0].is_cuda:
         raise RuntimeError(f"gradients on {grads[0].device}: disco_amd runs on the GPU only, there is no CPU fallback")
 
 
@@ -49,45 +49,10 @@ def _norm_type(norm_type) -> int:
     return p
 
 
-def _codes(tensors) -> array:
-    codes = _lib.DTYPES
-    return array("i", [codes[t.dtype] for t in tensors])
-
-
-def _launch(grads: Sequence[torch.Tensor], p: int, max_norm: Optional[float], out) -> torch.Tensor:
-    first = grads[0]
-    index = first.get_device()
-    if index != torch.cuda.current_device():
-        with torch.cuda.device(index):
-            return _launch(grads, p, max_norm, out)
-    lib = _lib.load()
-    n = len(grads)
-    src = array("Q", [g.data_ptr() for g in grads])
-    numel = array("q", [g.numel() for g in grads])
-    types = _codes(grads)
-    nb = lib.disco_grad_norm_workspace_bytes(n)
-    ws = torch.empty(nb, dtype=torch.uint8, device=first.device)
-    norm = torch.empty((), dtype=torch.float32, device=first.device)
-    stream = _lib.stream_of(index)
-    if max_norm is None:
-        status = lib.disco_grad_norm(src.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0], n, p, norm.data_ptr(),
-                                     ws.data_ptr(), nb, stream)
-        _lib.check(status, "disco_grad_norm")
-    else:
-        same = out is grads
-        dst = src if same else array("Q", [o.data_ptr() for o in out])
-        to = types if same else _codes(out)
-        status = lib.disco_grad_clip(src.buffer_info()[0], dst.buffer_info()[0], numel.buffer_info()[0], types.buffer_info()[0],
-                                     to.buffer_info()[0], n, p, max_norm, norm.data_ptr(), ws.data_ptr(), nb, stream)
-        if status == -1:
-            raise ValueError(_SHARED)
-        _lib.check(status, "disco_grad_clip")
-        # written behind autograd's back: whoever saved one of them must notice
-        try:
-            torch.autograd.graph.increment_version(out)
-        except RuntimeError:      # tensors made in inference mode keep no version
-            torch.autograd.graph.increment_version([o for o in out if not o.is_inference()])
-    return norm
+def _launch(grads: Sequence[torch.Tensor], out, p: int, max_norm: float) -> Optional[torch.Tensor]:
+    """The norm, and the clipping into ``out`` where that is given; None where the kernels do not read the tensors as they are."""
+    index = grads[0].get_device()
+    return _lib.torch_op("gradient_norm")(grads, out, p, max_norm, _lib.stream_of(index)) if index >= 0 else None
 
 
 def _dense(g: torch.Tensor) -> bool:
@@ -106,11 +71,14 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     """``(sum |g|^p)^(1/p)`` over every element of every tensor, p = ``norm_type`` in {1, 2, inf}; a float32 scalar on the
     device.  Sums run in float64 in a fixed order: nothing overflows in between, and the result does not vary."""
     p = _norm_type(norm_type)
-    grads = _tensors(grads)
-    _on_gpu(grads)
+    grads = _list(grads)
     if not grads:
         return torch.zeros((), dtype=torch.float32, device="cuda" if torch.cuda.is_available() else "cpu")
-    return _launch([g if _dense(g) else g.detach().contiguous() for g in grads], p, None, None)
+    norm = _launch(grads, None, p, 0.0)
+    if norm is None:
+        _check(grads)
+        norm = _launch([g if _dense(g) else g.detach().contiguous() for g in grads], None, p, 0.0)
+    return norm
 
 
 def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
@@ -125,30 +93,20 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must be a number that is not negative, got {max_norm}")
-    grads = _tensors(grads)
-    if out is None:
-        dst = grads
-    else:
-        dst = _tensors(out)
-        if len(dst) != len(grads):
-            raise ValueError(f"out has {len(dst)} tensors for {len(grads)} gradients")
-        f32 = torch.float32
-        if dst and dst[0].device != grads[0].device or any(
-                [o.shape != g.shape or (o.dtype is not f32 and o.dtype is not g.dtype) for g, o in zip(grads, dst)]):
-            for g, o in zip(grads, dst):
-                if o.shape == g.shape and o.device == g.device and o.dtype in (g.dtype, f32):
-                    continue
-                raise ValueError(f"out must have the gradients' shapes and device and their type or float32, got {tuple(o.shape)} "
-                                 f"{o.dtype} on {o.device} for {tuple(g.shape)} {g.dtype} on {g.device}")
-    _on_gpu(grads)
-    if not grads:
+    grads = _list(grads)
+    dst = grads if out is None else _list(out)
+    if not grads and not dst:
         return grad_norm(grads, norm_type)
     if error_if_nonfinite:
         norm = grad_norm(grads, norm_type)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"the norm of the gradients is {float(norm)}: they were not clipped")
-    if all([o.is_contiguous() for o in dst]) and (dst is grads or all([g.is_contiguous() for g in grads])):
-        return _launch(grads, p, max_norm, dst)
+    norm = _launch(grads, dst, p, max_norm) if grads else None
+    if norm is not None:
+        return norm
+    if len(dst) != len(grads):
+        raise ValueError(f"out has {len(dst)} tensors for {len(grads)} gradients")
+    _check(grads, dst)
     # the kernels walk memory in order: a pair that lies differently, or with gaps, goes through contiguous copies
     src, to, back = [], [], []
     for g, o in zip(grads, dst):
@@ -161,7 +119,9 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         src.append(g.detach().contiguous())
         to.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
         back.append((o, to[-1]))
-    norm = _launch(src, p, max_norm, to)
+    norm = _launch(src, to, p, max_norm)
+    if norm is None:
+        raise ValueError(_SHARED)
     with torch.no_grad():
         for o, t in back:
             o.copy_(t)

@@ -181,7 +181,9 @@ def test_residual_models_refuse_and_leave_the_others_alone():
 
 
 def test_the_torch_operator_is_built_and_bound():
-    op = _lib.residual_op()
+    op = _lib.torch_op("residual_norm")
     assert "libdisco_torch.so" in open("/proc/self/maps").read()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         op(torch.zeros(4, 8), None, None, None, None, None, None, None, 1 << 2, 1.0, 1e-5, 0)
+    norm = _lib.torch_op("gradient_norm")
+    assert norm([], None, 2, 0.0, 0) is None and norm([torch.zeros(3)], None, 2, 0.0, 0) is None
