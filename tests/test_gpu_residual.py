@@ -292,6 +292,15 @@ def test_broadcast_operands():
     near(gx, tuple(v.sum(0, keepdim=True) for v in want["x"]), "d_x")
     near(gg, tuple(v.sum(0, keepdim=True) for v in want["gate"]), "d_gate")
     near(gy, want["y"], "d_y")
+    # a gate that is one column of a wider matrix, and one row of gates for all rows
+    wide = torch.randn(30, 7, device=DEV)
+    s["t"]["gate"] = wide[:, 3:4]
+    near(call(s)[0], formula(s)["out"], "gate column")
+    got = train(s)[2]["gate"]
+    near(got, formula(s)["gate"], "d_gate column")
+    s["gate_kind"] = "full"
+    s["t"]["gate"] = torch.randn(1, 64, device=DEV).expand(30, 64)
+    check(s, what="repeated gates")
     # one scalar scale for all channels
     a = torch.full((), 0.7, device=DEV, requires_grad=True)
     out = ops.residual_norm(s["t"]["x"], s["t"]["y"], scale=a.expand(64))
@@ -319,6 +328,9 @@ def test_mixed_parameter_types_meet_in_float32():
 
 
 def test_empty_and_constant_rows():
+    x0, w0 = torch.empty(0, 5, device=DEV, requires_grad=True), torch.ones(5, device=DEV, requires_grad=True)
+    gx, gw = torch.autograd.grad(ops.row_norm(x0, w0).sum(), (x0, w0))
+    assert gx.shape == (0, 5) and torch.equal(gw, torch.zeros(5, device=DEV))
     s = make(0, 33)
     out, h, grads = train(s)
     assert out.shape == (0, 33) and h.shape == (0, 33) and grads["x"].shape == (0, 33) and grads["gate"].shape == (0, 33)
@@ -338,15 +350,17 @@ def test_empty_and_constant_rows():
     check(s)
 
 
-def test_nan_and_inf_stay_in_their_rows():
-    s = make(40, 96, seed=51)
+@pytest.mark.parametrize("stream,block", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("F", [96, 3, 50, 1200])
+def test_nan_and_inf_stay_in_their_rows(stream, block, F):
+    s = make(40, F, stream, block, seed=51)
     clean = train(s)
-    s["t"]["y"][3, 5], s["t"]["x"][7, 95], s["t"]["gate"][11, 0] = float("nan"), float("inf"), float("nan")
+    s["t"]["y"][3, F // 2], s["t"]["x"][7, F - 1], s["t"]["gate"][11, 0] = float("nan"), float("inf"), float("nan")
     out, h, grads = train(s)
     rest = [i for i in range(40) if i not in (3, 7, 11)]
     for a, b in ((out, clean[0]), (h, clean[1]), (grads["x"], clean[2]["x"]), (grads["y"], clean[2]["y"]), (grads["gate"], clean[2]["gate"])):
         assert torch.equal(a[rest], b[rest])
-    assert out[3].isnan().all() and h[3].isnan().all() and out[7, 95] == float("inf") and h[7].isnan().any()
+    assert out[3].isnan().all() and h[3].isnan().all() and out[7, F - 1] == float("inf") and h[7].isnan().any()
     assert out[11, 0].isnan() and torch.equal(out[11, 1:], clean[0][11, 1:]) and h[11].isnan().all()
     assert grads["pre_weight"].isnan().all()
     # a gate of plus / minus infinity is an open / closed gate
