@@ -69,7 +69,8 @@ def _dense(g: torch.Tensor) -> bool:
 
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """``(sum |g|^p)^(1/p)`` over every element of every tensor, p = ``norm_type`` in {1, 2, inf}; a float32 scalar on the
-    device.  Sums run in float64 in a fixed order: nothing overflows in between, and the result does not vary."""
+    device.  Sums run in float64 in a fixed order: nothing overflows in between (a norm beyond float32 is infinite), and the
+    result does not vary."""
     p = _norm_type(norm_type)
     grads = _list(grads)
     if not grads:
@@ -77,7 +78,7 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     norm = _launch(grads, None, p, 0.0)
     if norm is None:
         _check(grads)
-        norm = _launch([g if _dense(g) else g.detach().contiguous() for g in grads], None, p, 0.0)
+        norm = _launch([g.detach().contiguous() for g in grads], None, p, 0.0)
     return norm
 
 
@@ -86,9 +87,9 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     """Scales every gradient by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before (float32, on the device).
 
     In place by default; ``out`` names one destination per gradient, of its shape and either its type or float32 (the
-    buffers a mixed-precision optimiser reads).  Tensors that share memory are refused.  An infinite norm scales by zero
-    and a NaN norm makes every gradient NaN; with ``error_if_nonfinite`` such a norm raises RuntimeError and changes
-    nothing (this waits for the GPU)."""
+    buffers a mixed-precision optimiser reads).  Tensors that share memory are refused.  An infinite entry scales by zero
+    and a NaN makes every gradient NaN; with ``error_if_nonfinite`` a norm that is not finite in float32 raises
+    RuntimeError and changes nothing (this waits for the GPU)."""
     p = _norm_type(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
