@@ -4,10 +4,10 @@
 //   out  = g * min(1, max_norm / (norm + 1e-6))
 //
 // Bound by memory: the norm reads every gradient once (201 M float32 values: 141 us, 5.7 TB/s), clipping reads it again, since
-// no element may be scaled before the last one has been read, and writes it once.  The tensors are named in the launch's own arguments, up to a few hundred per
-// launch, so that no table is copied to the device and a launch can be captured.  Sums are float64 per lane: squares of
-// float32 values neither overflow nor vanish there, and one conversion and one fused add per element cost nothing next to
-// the read.  Every sum has a fixed order: the norm is the same from run to run.
+// no element may be scaled before the last one has been read, and writes it once.  The tensors are named in the launch's own
+// arguments, 136 a launch, so that no table is copied to the device and a launch can be captured.  Sums are float64 per lane:
+// squares of float32 values neither overflow nor vanish there, and one conversion and one fused add per element cost nothing
+// next to the read.  Every sum has a fixed order: the norm is the same from run to run.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
