@@ -115,7 +115,8 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
     Outputs r = ::forward(p, o, factor, eps, stream, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({o.x, o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, r.stats});
+    // without a next norm no gradient reads x: it is not kept, and may change
+    ctx->save_for_backward({p.pre ? o.x : Tensor(), o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, r.stats});
     // the node runs on its forward's stream, whichever one its caller is on
     ctx->saved_data["ints"] = std::vector<int64_t>{plan, stream};
     ctx->saved_data["floats"] = std::vector<double>{factor, eps};
@@ -133,13 +134,13 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Tensor dout = p.block ? rows(grads[0]) : Tensor(), dh = p.pre ? rows(grads[p.block ? 1 : 0]) : Tensor();
     if (!dout.defined() && !dh.defined()) return result;
     const variable_list s = ctx->get_saved_variables();
-    const Operands o{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7]};
+    const Operands o{p.pre ? s[0] : dout, s[1], s[2], s[3], s[4], s[5], s[6], s[7]};      // dout: of x's shape and type
     const c10::DeviceGuard guard(o.x.device());
     const int64_t n = o.x.size(0), width = o.x.size(1);
     // without a gradient of h the stream's gradient is that of out itself
     const bool through = !dh.defined();
     for (size_t i = 0, edge = 0; i < 8; ++i) {      // edges are numbered over the operands that are there
-      if (!s[i].defined() || !ctx->needs_input_grad(edge++)) continue;
+      if ((i > 0 && !s[i].defined()) || !ctx->needs_input_grad(edge++)) continue;
       if (through && (i == 0 || i >= 6)) continue;
       result[i] = at::empty(s[i].sizes(), s[i].options());
     }

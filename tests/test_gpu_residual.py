@@ -483,6 +483,25 @@ def test_what_autograd_keeps():
         assert ((a.double() - b).abs() <= C * (1 + b.abs().max())).all()
 
 
+@pytest.mark.parametrize("gate", [None, "row", "full"])
+def test_the_stream_may_change_where_no_norm_reads_it(gate):
+    s = make(20, 30, pre=None, gate=gate, act=gate and "sigmoid")
+    want = train(s, ("out",))
+    t = {k: v.clone().requires_grad_() for k, v in s["t"].items()}
+    x = t["x"] * 1.0
+    out = call(s, {**t, "x": x})
+    out = out[0] if isinstance(out, tuple) else out
+    x.detach().add_(1.0)
+    got = torch.autograd.grad((out * s["dout"]).sum(), list(t.values()))
+    for k, g in zip(t, got):
+        assert torch.equal(g, want[2][k]), k
+    x = t["x"] * 1.0
+    out, h = call(make(20, 30), {**make(20, 30)["t"], "x": x})
+    x.detach().add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        (out.sum() + h.sum()).backward()
+
+
 def test_second_derivatives_are_refused():
     s = make(4, 16, gate=None, act=None)
     t = {k: v.clone().requires_grad_() for k, v in s["t"].items()}
