@@ -87,9 +87,10 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     """Scales every gradient by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before (float32, on the device).
 
     In place by default; ``out`` names one destination per gradient, of its shape and either its type or float32 (the
-    buffers a mixed-precision optimiser reads).  Tensors that share memory are refused.  An infinite entry scales by zero
-    and a NaN makes every gradient NaN; with ``error_if_nonfinite`` a norm that is not finite in float32 raises
-    RuntimeError and changes nothing (this waits for the GPU)."""
+    buffers a mixed-precision optimiser reads).  Dense tensors that share memory are refused; views with gaps are read before
+    anything is written, so that no element is scaled twice.  An infinite entry scales by zero and a NaN makes every
+    gradient NaN; with ``error_if_nonfinite`` a norm that is not finite in float32 raises RuntimeError and changes nothing
+    (this waits for the GPU)."""
     p = _norm_type(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:

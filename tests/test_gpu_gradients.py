@@ -161,6 +161,18 @@ def test_views_of_one_buffer_and_shared_memory():
         ops.clip_grads([flat[:10]], 1.0, out=[flat[1:11]])
 
 
+def test_views_with_gaps_that_share_memory_are_scaled_once():
+    hole = torch.randn(64, 100, device=DEV)
+    keep = hole.clone()
+    for views in (lambda t: [t[:, 10:58], t[:, 10:58]], lambda t: [t[:, 10:58], t[:, 40:90]], lambda t: [t[:, ::2], t[:, 1::2]],
+                  lambda t: [t[:, 10:58], t[20:30]]):
+        hole.copy_(keep)
+        before, after = views(keep), views(hole)
+        want = norm64(before, 2)
+        check_norm(ops.clip_grads(after, 1.0), want)
+        check_clip(before, after, 1.0, want)
+
+
 def test_parameters():
     m = torch.nn.Sequential(torch.nn.Linear(40, 30), torch.nn.BatchNorm1d(30), torch.nn.Linear(30, 1)).to(DEV)
     unused = torch.nn.Parameter(torch.ones(5, device=DEV))
