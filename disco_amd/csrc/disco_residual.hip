@@ -90,6 +90,12 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   if (a.db2) param_put(a.db2, a.param_type, c, P4);
 }
 
+// Zeros into rows of `width` elements, for a gradient that nothing flows into.
+template <typename T>
+__global__ __launch_bounds__(256) void k_residual_zero(T* p, int64_t rows, int64_t width, int64_t ld) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * width; i += (int64_t)gridDim.x * 256) p[i / width * ld + i % width] = (T)0.0f;
+}
+
 static int pair_of(int stream_type, int block_type) {
   if (stream_type == block_type) return stream_type == DISCO_F32 ? kPairF32 : stream_type == DISCO_F16 ? kPairF16 : stream_type == DISCO_BF16 ? kPairBF16 : -1;
   if (stream_type == DISCO_F32) return block_type == DISCO_F16 ? kPairF32F16 : block_type == DISCO_BF16 ? kPairF32BF16 : -1;
@@ -211,13 +217,22 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
   const ResidualShape s = residual_shape(F, d->block_type != DISCO_F32);
   const unsigned grid = backward_grid(n, s, residual_mode(d->has_block, d->gate_kind));
   const size_t need = (size_t)grid * 4 * (size_t)F * sizeof(float);
-  if (a.partials && n > 0 && (!workspace || workspace_bytes < need)) return DISCO_EWORKSPACE;
+  // The norm alone without a gradient of h: every gradient is zero, and neither x nor the statistics are there to be read.
+  const bool nothing = !d->has_block && !g->dh;
+  const int64_t summed = nothing ? 0 : n;
+  if (a.partials && summed > 0 && (!workspace || workspace_bytes < need)) return DISCO_EWORKSPACE;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   a.stats = const_cast<float*>(stats);
   a.dout = g->dout; a.lddo = g->ld_dout; a.dh = g->dh; a.lddh = g->ld_dh;
   a.dx = g->dx; a.lddx = g->ld_dx; a.dy = g->dy; a.lddy = g->ld_dy; a.dg = channel ? nullptr : g->dgate; a.lddg = g->ld_dgate;
   a.partial = a.partials ? static_cast<float*>(workspace) : nullptr;
-  if (n > 0 && (a.dx || a.dy || a.dg || a.partials)) {
+  if (nothing && a.dx && n > 0) {
+    const dim3 blocks((unsigned)std::min<int64_t>((n * F + 255) / 256, 4096));
+    if (d->stream_type == DISCO_F32) hipLaunchKernelGGL(k_residual_zero<float>, blocks, dim3(256), 0, stream, static_cast<float*>(a.dx), n, F, a.lddx);
+    else hipLaunchKernelGGL(k_residual_zero<_Float16>, blocks, dim3(256), 0, stream, static_cast<_Float16*>(a.dx), n, F, a.lddx);      // bfloat16 too
+    DISCO_CHECK_LAUNCH();
+  }
+  if (summed > 0 && (a.dx || a.dy || a.dg || a.partials)) {
     int r;
     switch (pair_of(d->stream_type, d->block_type)) {
       case kPairF32: r = residual_backward<kPairF32>(a, grid, stream); break;
@@ -230,7 +245,7 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
   }
   if (!a.partials) return DISCO_OK;
   FinishArgs f{};
-  f.partial = a.partial; f.groups = n > 0 ? grid : 0; f.width = (int)F; f.partials = a.partials; f.param_type = d->param_type;
+  f.partial = a.partial; f.groups = summed > 0 ? grid : 0; f.width = (int)F; f.partials = a.partials; f.param_type = d->param_type;
   f.channel = channel; f.act = d->gate_act; f.scale = d->scale;
   f.w1 = d->post_weight; f.b1 = d->post_bias; f.lam = d->scale_vector; f.g = channel ? d->gate : nullptr;
   f.dw1 = g->dpost_weight; f.db1 = g->dpost_bias; f.dw2 = g->dpre_weight; f.db2 = g->dpre_bias; f.dlam = g->dscale;

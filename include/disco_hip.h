@@ -388,7 +388,8 @@ typedef struct disco_residual_norm {
 } disco_residual_norm;
 
 /* Gradients of the outputs (NULL: zero) and of the inputs (NULL: not wanted; a gradient of an input that the descriptor
- * leaves away is refused).  dgate has the gate's shape; the vectors' gradients have the parameter type. */
+ * leaves away is refused).  The norm alone (has_block = 0) without dh reads nothing and gives zeros.  dgate has the gate's
+ * shape; the vectors' gradients have the parameter type. */
 typedef struct disco_residual_norm_grads {
   const void *dout, *dh;
   void *dx, *dy, *dgate;

@@ -548,3 +548,18 @@ def test_drawn_cases(case):
     s = make(n, F, stream, block, ["f32", block][r.integers(2)], [None, "rms", "layer"][r.integers(3)], [None, "rms", "layer"][r.integers(3)],
              gate, [None, "sigmoid", "tanh"][r.integers(3)], ["vector", "number"][r.integers(2)], bool(r.integers(2)), seed=case)
     check(s, what=f"{case}: n={n} F={F} {stream}/{block}")
+
+
+@pytest.mark.parametrize("n,F,ld", [(1, 1, 1), (5, 7, 11), (300, 602, 610), (70000, 3, 4)])
+@pytest.mark.parametrize("stream,block", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16")])
+def test_the_norm_without_a_gradient_has_zero_gradients(n, F, ld, stream, block):
+    """C entry, norm alone, dh NULL ("NULL: zero"): x, the statistics and the workspace are not there, and nothing is read."""
+    from disco_amd import _lib
+    lib = _lib.load()
+    dx = torch.full((n + 1, ld), 7.0, dtype=T[stream], device=DEV)
+    w, dw, db = (torch.full((F,), 7.0, device=DEV) for _ in range(3))
+    d = _lib.ResidualNorm(rows=n, width=F, ldx=F, has_block=0, pre_norm=2, pre_weight=w.data_ptr(), pre_bias=w.data_ptr(), scale=1.0, eps=EPS,
+                          stream_type=_lib.DTYPES[T[stream]], block_type=_lib.DTYPES[T[block]])
+    g = _lib.ResidualNormGrads(dx=dx.data_ptr(), ld_dx=ld, dpre_weight=dw.data_ptr(), dpre_bias=db.data_ptr())
+    _lib.check(lib.disco_residual_norm_backward(d, None, g, None, 0, _lib.current_stream(dx.device)), "backward")
+    assert not dx[:n, :F].any() and (dx[n:] == 7).all() and (dx[:, F:] == 7).all() and not dw.any() and not db.any()
