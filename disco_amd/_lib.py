@@ -198,8 +198,3 @@ def ptr(t) -> int | None:
 
 def current_stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
-
-
-def stream_of(index: int) -> int:
-    """:func:`current_stream` of a device by its index, without the Stream object around it: calls of a few microseconds."""
-    return torch._C._cuda_getCurrentRawStream(index)

@@ -40,15 +40,16 @@ def _newest_source_mtime() -> float:
 
 
 def build_torch_lib(force: bool = False) -> str:
-    """libdisco_torch.so: the autograd node of the residual join, host code against torch's own headers and libraries."""
+    """libdisco_torch.so: the torch operators of the residual join and the gradient norm, host code against torch's own headers
+    and libraries."""
     out, src = lib_path("libdisco_torch.so"), os.path.join(CSRC, "disco_torch.cpp")
     needs = [src, os.path.join(ROOT, "include", "disco_hip.h"), os.path.abspath(__file__)]
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(map(os.path.getmtime, needs)):
         return out
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-                           *("-I" + p for p in include_paths()), src, "-o", out, *("-L" + p for p in library_paths()), "-ltorch", "-ltorch_cpu", "-lc10"])
+    subprocess.check_call(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                           *("-I" + p for p in include_paths("cuda")), src, "-o", out, *("-L" + p for p in library_paths()), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"])
     return out
 
 

@@ -7,6 +7,7 @@
 // backward reads.  A list of gradients is read here too: an attribute of every tensor costs in Python what a launch does (norm
 // and clipping of ten: 17 and 26 us, 12 and 13 here).  The entries' addresses come from the loaded library (bind), so there is one copy of it in the process.
 #include <ATen/ATen.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -43,6 +44,10 @@ void bind(int64_t forward, int64_t backward, int64_t workspace, int64_t status, 
   g_workspace = reinterpret_cast<decltype(g_workspace)>(workspace);
   g_status = reinterpret_cast<decltype(g_status)>(status);
 }
+
+// The stream that is current where the call happens.  (A handle among the operator's arguments would become a constant of a
+// traced module, which then launches on the stream of its tracing.)
+void* stream_of(const at::Device& device) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream(); }
 
 void check(int status, const char* what) { TORCH_CHECK(status == DISCO_OK, what, ": ", g_status(status)); }
 
@@ -88,14 +93,14 @@ struct Outputs { Tensor out, h, stats; };
 
 // Output rows lie densely: columns that nothing writes between them leave cache lines half written (the norm of 2.4 M rows of
 // 41 floats: 268 us with rows padded to 44, 170 dense).
-Outputs forward(const Plan& p, const Operands& o, double scale, double eps, int64_t stream, bool keep) {
+Outputs forward(const Plan& p, const Operands& o, double scale, double eps, bool keep) {
   const c10::DeviceGuard guard(o.x.device());
   Outputs r;
   if (p.block) r.out = at::empty(o.x.sizes(), o.x.options());
   if (p.pre) r.h = at::empty(o.x.sizes(), o.x.options().dtype(type_of(p.block_type)));
   if (keep) r.stats = at::empty({4 * o.x.size(0)}, o.x.options().dtype(at::kFloat));
   const disco_residual_norm d = describe(p, o, scale, eps);
-  check(g_forward(&d, write(r.out), pitch(r.out, 0), write(r.h), pitch(r.h, 0), static_cast<float*>(write(r.stats)), reinterpret_cast<void*>(stream)),
+  check(g_forward(&d, write(r.out), pitch(r.out, 0), write(r.h), pitch(r.h, 0), static_cast<float*>(write(r.stats)), stream_of(o.x.device())),
         "disco_residual_norm_forward");
   return r;
 }
@@ -110,15 +115,14 @@ Tensor rows(const Tensor& t) {
 class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1,
-                               const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t stream) {
+                               const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps) {
     const Plan p(plan);
     const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
-    Outputs r = ::forward(p, o, factor, eps, stream, true);
+    Outputs r = ::forward(p, o, factor, eps, true);
     ctx->set_materialize_grads(false);
     // without a next norm no gradient reads x: it is not kept, and may change
     ctx->save_for_backward({p.pre ? o.x : Tensor(), o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, r.stats});
-    // the node runs on its forward's stream, whichever one its caller is on
-    ctx->saved_data["ints"] = std::vector<int64_t>{plan, stream};
+    ctx->saved_data["plan"] = plan;
     ctx->saved_data["floats"] = std::vector<double>{factor, eps};
     variable_list outputs;
     if (p.block) outputs.push_back(r.out);
@@ -127,10 +131,9 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list result(12);
-    const auto ints = ctx->saved_data["ints"].toIntVector();
+    variable_list result(11);
     const auto floats = ctx->saved_data["floats"].toDoubleVector();
-    const Plan p(ints[0]);
+    const Plan p(ctx->saved_data["plan"].toInt());
     const Tensor dout = p.block ? rows(grads[0]) : Tensor(), dh = p.pre ? rows(grads[p.block ? 1 : 0]) : Tensor();
     if (!dout.defined() && !dh.defined()) return result;
     const variable_list s = ctx->get_saved_variables();
@@ -153,12 +156,13 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     g.dpost_weight = write(result[4]); g.dpost_bias = write(result[5]); g.dpre_weight = write(result[6]); g.dpre_bias = write(result[7]);
     g.ld_dout = pitch(dout, width); g.ld_dh = pitch(dh, width); g.ld_dx = pitch(result[0], width); g.ld_dy = pitch(result[1], width);
     g.ld_dgate = pitch(result[2], width);
-    check(g_backward(&d, static_cast<const float*>(read(s[8])), &g, write(ws), bytes, reinterpret_cast<void*>(ints[1])), "disco_residual_norm_backward");
+    // autograd makes the forward's stream current for its node, whichever one the caller of the backward is on
+    check(g_backward(&d, static_cast<const float*>(read(s[8])), &g, write(ws), bytes, stream_of(o.x.device())), "disco_residual_norm_backward");
     if (through && ctx->needs_input_grad(0)) result[0] = dout;
     if (at::GradMode::is_enabled()) {      // the gradients have no formula of their own: whoever differentiates them is told
       for (Tensor& t : result)
         if (t.defined()) t = t.detach().requires_grad_();
-      const auto refuse = std::make_shared<torch::autograd::DelayedError>("residual_norm has no second derivatives", 12);
+      const auto refuse = std::make_shared<torch::autograd::DelayedError>("residual_norm has no second derivatives", 11);
       return (*refuse)(std::move(result));
     }
     return result;
@@ -166,16 +170,16 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
 };
 
 std::vector<Tensor> residual_norm(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1,
-                                  const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t stream) {
+                                  const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t /*stream: unused*/) {
   TORCH_CHECK(g_forward && g_backward && g_workspace && g_status, "disco_torch: not bound to libdisco_hip.so");
   TORCH_CHECK(x.is_cuda(), "x is on ", x.device(), ": disco_amd runs on the GPU only, there is no CPU fallback");
   const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
   bool grad = false;
   if (at::GradMode::is_enabled())
     for (const Tensor* t : {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2}) grad = grad || (t->defined() && t->requires_grad());
-  if (grad) return ResidualNorm::apply(x, y, gate, scale, w1, b1, w2, b2, plan, factor, eps, stream);
+  if (grad) return ResidualNorm::apply(x, y, gate, scale, w1, b1, w2, b2, plan, factor, eps);
   const Plan p(plan);
-  const Outputs r = forward(p, o, factor, eps, stream, false);
+  const Outputs r = forward(p, o, factor, eps, false);
   std::vector<Tensor> outputs;
   if (p.block) outputs.push_back(r.out);
   if (p.pre) outputs.push_back(r.h);
@@ -191,7 +195,7 @@ bool known(const Tensor& t) {
 // tensors are not what the kernels read -- on one GPU, of a known type, without gaps, each output of its gradient's shape,
 // strides and type or float32, none sharing memory: gradients.py then says what is wrong, or makes copies.
 std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out, int64_t norm_type, double max_norm,
-                                    int64_t stream) {
+                                    int64_t /*stream: unused*/) {
   TORCH_CHECK(g_norm && g_clip && g_norm_workspace, "disco_torch: not bound to libdisco_hip.so");
   const size_t n = grads.size();
   if (n == 0 || !grads[0].is_cuda() || (out && out->size() != n)) return std::nullopt;
@@ -222,12 +226,12 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
   const Tensor ws = at::empty({(int64_t)bytes}, options.dtype(at::kByte)), norm = at::empty({}, options.dtype(at::kFloat));
   float* to = static_cast<float*>(norm.mutable_data_ptr());
   if (!out) {
-    check(g_norm(src.data(), numel.data(), type.data(), (int64_t)n, (int)norm_type, to, write(ws), bytes, reinterpret_cast<void*>(stream)),
+    check(g_norm(src.data(), numel.data(), type.data(), (int64_t)n, (int)norm_type, to, write(ws), bytes, stream_of(device)),
           "disco_grad_norm");
     return norm;
   }
   const int status = g_clip(src.data(), dst.data(), numel.data(), type.data(), out_type.data(), (int64_t)n, (int)norm_type, max_norm, to, write(ws),
-                            bytes, reinterpret_cast<void*>(stream));
+                            bytes, stream_of(device));
   if (status == DISCO_EINVAL) return std::nullopt;
   check(status, "disco_grad_clip");
   for (const Tensor& o : *out)      // written behind autograd's back: whoever saved one of them must notice
@@ -237,11 +241,12 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
 
 }  // namespace
 
+// `stream` is not read: it stands for callers that still pass one.
 TORCH_LIBRARY(disco_amd, m) {
   m.def("bind(int forward, int backward, int workspace, int status, int norm, int clip, int norm_workspace) -> ()", &bind);
-  m.def("gradient_norm(Tensor[] grads, Tensor[]? out, int norm_type, float max_norm, int stream) -> Tensor?", &gradient_norm);
+  m.def("gradient_norm(Tensor[] grads, Tensor[]? out, int norm_type, float max_norm, int stream=0) -> Tensor?", &gradient_norm);
   m.def(
       "residual_norm(Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? post_weight, Tensor? post_bias, Tensor? pre_weight, "
-      "Tensor? pre_bias, int plan, float factor, float eps, int stream) -> Tensor[]",
+      "Tensor? pre_bias, int plan, float factor, float eps, int stream=0) -> Tensor[]",
       &residual_norm);
 }

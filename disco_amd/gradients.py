@@ -51,8 +51,7 @@ def _norm_type(norm_type) -> int:
 
 def _launch(grads: Sequence[torch.Tensor], out, p: int, max_norm: float) -> Optional[torch.Tensor]:
     """The norm, and the clipping into ``out`` where that is given; None where the kernels do not read the tensors as they are."""
-    index = grads[0].get_device()
-    return _lib.torch_op("gradient_norm")(grads, out, p, max_norm, _lib.stream_of(index)) if index >= 0 else None
+    return _lib.torch_op("gradient_norm")(grads, out, p, max_norm)
 
 
 def _dense(g: torch.Tensor) -> bool:

@@ -92,8 +92,7 @@ def _run(plan, x, y, gate, scale, eps, vectors):
         gate = _vector(channel, dtype)
     elif gate is not None and gate.shape[1] > 1:
         gate = _rows(gate)
-    return _lib.torch_op("residual_norm")(_rows(x), None if y is None else _rows(y), gate, *[_vector(v, dtype) for _, v in rest], options, scale, eps,
-                              _lib.stream_of(x.get_device()))
+    return _lib.torch_op("residual_norm")(_rows(x), None if y is None else _rows(y), gate, *[_vector(v, dtype) for _, v in rest], options, scale, eps)
 
 
 def row_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, kind: str = "layer",

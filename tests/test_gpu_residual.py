@@ -563,3 +563,19 @@ def test_the_norm_without_a_gradient_has_zero_gradients(n, F, ld, stream, block)
     g = _lib.ResidualNormGrads(dx=dx.data_ptr(), ld_dx=ld, dpre_weight=dw.data_ptr(), dpre_bias=db.data_ptr())
     _lib.check(lib.disco_residual_norm_backward(d, None, g, None, 0, _lib.current_stream(dx.device)), "backward")
     assert not dx[:n, :F].any() and (dx[n:] == 7).all() and (dx[:, F:] == 7).all() and not dw.any() and not db.any()
+
+
+def test_a_traced_call_runs_on_the_stream_of_its_caller():
+    """Traced on one stream, called on another behind work that is still running there: it waits for that work."""
+    x, w = torch.zeros(64, 48, device=DEV), torch.randn(48, device=DEV)
+    new = torch.randn(64, 48, device=DEV)
+    f = torch.jit.trace(lambda v: ops.row_norm(v, w) + ops.residual_norm(v, v, post="rms"), x)
+    want = ops.row_norm(new, w) + ops.residual_norm(new, new, post="rms")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        x.copy_(new)
+        got = f(x)
+    side.synchronize()
+    assert torch.equal(got, want)

@@ -187,3 +187,10 @@ def test_the_torch_operator_is_built_and_bound():
         op(torch.zeros(4, 8), None, None, None, None, None, None, None, 1 << 2, 1.0, 1e-5, 0)
     norm = _lib.torch_op("gradient_norm")
     assert norm([], None, 2, 0.0, 0) is None and norm([torch.zeros(3)], None, 2, 0.0, 0) is None
+
+
+def test_the_torch_operators_take_no_stream():
+    """A stream handle among the arguments would be a constant of a traced module: the operators read the current stream."""
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        _lib.torch_op("residual_norm")(torch.zeros(4, 8), None, None, None, None, None, None, None, 1 << 2, 1.0, 1e-5)
+    assert _lib.torch_op("gradient_norm")([torch.zeros(3)], None, 2, 0.0) is None
