@@ -49,6 +49,11 @@ void bind(int64_t forward, int64_t backward, int64_t workspace, int64_t status, 
 // traced module, which then launches on the stream of its tracing.)
 void* stream_of(const at::Device& device) { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(device.index()).stream(); }
 
+// Without this a tensor that carries a tangent but needs no gradient would come back without one.
+void refuse_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivatives");
+}
+
 void check(int status, const char* what) { TORCH_CHECK(status == DISCO_OK, what, ": ", g_status(status)); }
 
 // What a call does besides its tensors, as residual.py packs it: two bits each of the post norm, the pre norm, the gate, its
@@ -172,11 +177,14 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
 std::vector<Tensor> residual_norm(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1,
                                   const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t /*stream: unused*/) {
   TORCH_CHECK(g_forward && g_backward && g_workspace && g_status, "disco_torch: not bound to libdisco_hip.so");
-  TORCH_CHECK(x.is_cuda(), "x is on ", x.device(), ": disco_amd runs on the GPU only, there is no CPU fallback");
   const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
   bool grad = false;
-  if (at::GradMode::is_enabled())
-    for (const Tensor* t : {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2}) grad = grad || (t->defined() && t->requires_grad());
+  for (const Tensor* t : {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2}) {
+    refuse_tangent(*t, "residual_norm");
+    grad = grad || (t->defined() && t->requires_grad());
+  }
+  TORCH_CHECK(x.is_cuda(), "x is on ", x.device(), ": disco_amd runs on the GPU only, there is no CPU fallback");
+  grad = grad && at::GradMode::is_enabled();
   if (grad) return ResidualNorm::apply(x, y, gate, scale, w1, b1, w2, b2, plan, factor, eps);
   const Plan p(plan);
   const Outputs r = forward(p, o, factor, eps, false);
@@ -197,6 +205,9 @@ bool known(const Tensor& t) {
 std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out, int64_t norm_type, double max_norm,
                                     int64_t /*stream: unused*/) {
   TORCH_CHECK(g_norm && g_clip && g_norm_workspace, "disco_torch: not bound to libdisco_hip.so");
+  for (const Tensor& t : grads) refuse_tangent(t, "gradient_norm");
+  if (out)
+    for (const Tensor& t : *out) refuse_tangent(t, "gradient_norm");
   const size_t n = grads.size();
   if (n == 0 || !grads[0].is_cuda() || (out && out->size() != n)) return std::nullopt;
   const auto device = grads[0].device();

@@ -579,3 +579,16 @@ def test_a_traced_call_runs_on_the_stream_of_its_caller():
         got = f(x)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+def test_forward_mode_derivatives_are_refused():
+    import torch.autograd.forward_ad as fwad
+    x, w = torch.randn(4, 8, device=DEV), torch.randn(8, device=DEV)
+    with fwad.dual_level():
+        d, dw = fwad.make_dual(x, torch.ones_like(x)), fwad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: ops.row_norm(d), lambda: ops.row_norm(x, dw), lambda: ops.residual_norm(x, d), lambda: ops.residual_norm(x, x, gate=dw),
+                     lambda: ops.residual_norm(x, x, gate=d[:, :1]), lambda: ops.residual_norm(x, x, scale=dw.half()), lambda: ops.grad_norm([x, d]),
+                     lambda: ops.grad_norm(d[:, ::2]), lambda: ops.clip_grads([x], 1.0, out=[d])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+    ops.row_norm(d), ops.row_norm(x, dw)      # outside of the level they are ordinary tensors

@@ -194,3 +194,18 @@ def test_the_torch_operators_take_no_stream():
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         _lib.torch_op("residual_norm")(torch.zeros(4, 8), None, None, None, None, None, None, None, 1 << 2, 1.0, 1e-5)
     assert _lib.torch_op("gradient_norm")([torch.zeros(3)], None, 2, 0.0) is None
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent on a tensor that needs no gradient must not be dropped without a word."""
+    import torch.autograd.forward_ad as fwad
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    with fwad.dual_level():
+        d, dw = fwad.make_dual(x, torch.ones_like(x)), fwad.make_dual(w, torch.ones_like(w))
+        op, norm = _lib.torch_op("residual_norm"), _lib.torch_op("gradient_norm")
+        for args in ((d, None, None, None, None, None, None, None), (x, d, None, None, None, None, None, None), (x, None, None, None, None, None, dw, None)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                op(*args, 1 << 2, 1.0, 1e-5)
+        for grads, out in (([x, d], None), ([x, x], [d, x])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                norm(grads, out, 2, 1.0)
