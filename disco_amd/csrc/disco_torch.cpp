@@ -94,20 +94,38 @@ disco_residual_norm describe(const Plan& p, const Operands& o, double scale, dou
   return d;
 }
 
-struct Outputs { Tensor out, h, stats; };
+void bound() { TORCH_CHECK(g_forward && g_backward && g_workspace && g_status && g_norm && g_clip && g_norm_workspace, "disco_torch: not bound to libdisco_hip.so"); }
 
-// Output rows lie densely: columns that nothing writes between them leave cache lines half written (the norm of 2.4 M rows of
-// 41 floats: 268 us with rows padded to 44, 170 dense).
-Outputs forward(const Plan& p, const Operands& o, double scale, double eps, bool keep) {
-  const c10::DeviceGuard guard(o.x.device());
-  Outputs r;
-  if (p.block) r.out = at::empty(o.x.sizes(), o.x.options());
-  if (p.pre) r.h = at::empty(o.x.sizes(), o.x.options().dtype(type_of(p.block_type)));
-  if (keep) r.stats = at::empty({4 * o.x.size(0)}, o.x.options().dtype(at::kFloat));
-  const disco_residual_norm d = describe(p, o, scale, eps);
-  check(g_forward(&d, write(r.out), pitch(r.out, 0), write(r.h), pitch(r.h, 0), static_cast<float*>(write(r.stats)), stream_of(o.x.device())),
+// ---- operators of the dispatcher: what a tracer, a fake tensor or a mode sees of a call ---------------------------------
+// A call that went to the kernels around the dispatcher would leave nothing behind in a trace but its uninitialised outputs.
+
+// out, h and, where the backward wants them, the rows' statistics.  Output rows lie densely: columns that nothing writes
+// between them leave cache lines half written (the norm of 2.4 M rows of 41 floats: 268 us with rows padded to 44, 170 dense).
+variable_list forward_outputs(const Plan& p, const Tensor& x, bool keep) {
+  variable_list r;
+  if (p.block) r.push_back(at::empty_symint(x.sym_sizes(), x.options()));
+  if (p.pre) r.push_back(at::empty_symint(x.sym_sizes(), x.options().dtype(type_of(p.block_type))));
+  if (keep) r.push_back(at::empty_symint({4 * x.sym_size(0)}, x.options().dtype(at::kFloat)));
+  return r;
+}
+
+variable_list forward_op(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1, const Maybe& w2,
+                         const Maybe& b2, int64_t plan, double factor, double eps, bool keep) {
+  bound();
+  const Plan p(plan);
+  const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
+  const c10::DeviceGuard guard(x.device());
+  variable_list r = forward_outputs(p, x, keep);
+  const Tensor out = p.block ? r[0] : Tensor(), h = p.pre ? r[p.block] : Tensor(), stats = keep ? r.back() : Tensor();
+  const disco_residual_norm d = describe(p, o, factor, eps);
+  check(g_forward(&d, write(out), pitch(out, 0), write(h), pitch(h, 0), static_cast<float*>(write(stats)), stream_of(x.device())),
         "disco_residual_norm_forward");
   return r;
+}
+
+variable_list forward_meta(const Tensor& x, const Maybe&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, const Maybe&, int64_t plan,
+                           double, double, bool keep) {
+  return forward_outputs(Plan(plan), x, keep);
 }
 
 // Rows with unit column stride that do not overlap, or one row for all: the tensor or a copy.
@@ -117,52 +135,148 @@ Tensor rows(const Tensor& t) {
   return (width > 1 && c != 1) || (n > 1 && r > 0 && r < width) ? t.contiguous() : t;
 }
 
+// The operands' gradients that `wanted` names (a bit for each operand, in the operator's order), in that order.
+variable_list backward_outputs(const Operands& o, int64_t wanted) {
+  variable_list r;
+  const Tensor* all[] = {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2};
+  for (int i = 0; i < 8; ++i)
+    if (wanted >> i & 1) r.push_back(at::empty_symint(all[i]->sym_sizes(), all[i]->options()));
+  return r;
+}
+
+variable_list backward_op(const Maybe& dout_, const Maybe& dh_, const Maybe& stats, const Maybe& x, const Maybe& y, const Maybe& gate, const Maybe& scale,
+                          const Maybe& w1, const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t wanted) {
+  bound();
+  const Plan p(plan);
+  const Tensor dout = rows(dout_.value_or(Tensor())), dh = rows(dh_.value_or(Tensor()));
+  const Operands o = operands(x.value_or(dout), y, gate, scale, w1, b1, w2, b2);      // dout: of x's shape and type
+  const c10::DeviceGuard guard(o.x.device());
+  const int64_t n = o.x.size(0), width = o.x.size(1);
+  variable_list r = backward_outputs(o, wanted);
+  size_t next = 0;
+  const auto gradient = [&](int i) { return wanted >> i & 1 ? r[next++] : Tensor(); };
+  const Tensor dx = gradient(0), dy = gradient(1), dgate = gradient(2), dscale = gradient(3), dw1 = gradient(4), db1 = gradient(5), dw2 = gradient(6),
+               db2 = gradient(7);
+  const size_t bytes = g_workspace(n, width);
+  const Tensor ws = at::empty({(int64_t)bytes}, o.x.options().dtype(at::kByte));
+  const disco_residual_norm d = describe(p, o, factor, eps);
+  disco_residual_norm_grads g{};
+  g.dout = read(dout); g.dh = read(dh);
+  g.dx = write(dx); g.dy = write(dy); g.dgate = write(dgate); g.dscale = write(dscale);
+  g.dpost_weight = write(dw1); g.dpost_bias = write(db1); g.dpre_weight = write(dw2); g.dpre_bias = write(db2);
+  g.ld_dout = pitch(dout, width); g.ld_dh = pitch(dh, width); g.ld_dx = pitch(dx, width); g.ld_dy = pitch(dy, width); g.ld_dgate = pitch(dgate, width);
+  // autograd makes the forward's stream current for its node, whichever one the caller of the backward is on
+  check(g_backward(&d, static_cast<const float*>(read(stats.value_or(Tensor()))), &g, write(ws), bytes, stream_of(o.x.device())),
+        "disco_residual_norm_backward");
+  return r;
+}
+
+variable_list backward_meta(const Maybe& dout, const Maybe&, const Maybe&, const Maybe& x, const Maybe& y, const Maybe& gate, const Maybe& scale,
+                            const Maybe& w1, const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t, double, double, int64_t wanted) {
+  return backward_outputs(operands(x.has_value() ? *x : *dout, y, gate, scale, w1, b1, w2, b2), wanted);
+}
+
+// The tensors of a list as the C entries take them.
+struct List {
+  std::vector<const void*> src;
+  std::vector<void*> dst;
+  std::vector<int64_t> numel;
+  std::vector<int> type, out_type;
+  Tensor ws, norm;
+  List(at::TensorList grads, const at::TensorList* out) : src(grads.size()), dst(out ? grads.size() : 0), numel(grads.size()), type(grads.size()),
+                                                          out_type(out ? grads.size() : 0) {
+    bound();
+    const auto options = at::TensorOptions().device(grads[0].device());
+    ws = at::empty({(int64_t)g_norm_workspace((int64_t)grads.size())}, options.dtype(at::kByte));
+    norm = at::empty({}, options.dtype(at::kFloat));
+    for (size_t i = 0; i < grads.size(); ++i) {
+      src[i] = grads[i].const_data_ptr();
+      numel[i] = grads[i].numel();
+      type[i] = type_code(grads[i]);
+      if (!out) continue;
+      dst[i] = (*out)[i].mutable_data_ptr();
+      out_type[i] = type_code((*out)[i]);
+    }
+  }
+};
+
+Tensor norm_op(at::TensorList grads, int64_t norm_type) {
+  const c10::DeviceGuard guard(grads[0].device());
+  const List l(grads, nullptr);
+  check(g_norm(l.src.data(), l.numel.data(), l.type.data(), (int64_t)grads.size(), (int)norm_type, static_cast<float*>(write(l.norm)), write(l.ws),
+               (size_t)l.ws.numel(), stream_of(grads[0].device())), "disco_grad_norm");
+  return l.norm;
+}
+
+Tensor clip_op(at::TensorList grads, at::TensorList out, int64_t norm_type, double max_norm) {
+  const c10::DeviceGuard guard(grads[0].device());
+  const List l(grads, &out);
+  const int status = g_clip(l.src.data(), l.dst.data(), l.numel.data(), l.type.data(), l.out_type.data(), (int64_t)grads.size(), (int)norm_type, max_norm,
+                            static_cast<float*>(write(l.norm)), write(l.ws), (size_t)l.ws.numel(), stream_of(grads[0].device()));
+  TORCH_CHECK_VALUE(status != DISCO_EINVAL, "clip_grads: two tensors share memory; each gradient may be scaled only once");
+  check(status, "disco_grad_clip");
+  return l.norm;
+}
+
+Tensor norm_meta(at::TensorList grads, int64_t) { return at::empty({}, grads[0].options().dtype(at::kFloat)); }
+Tensor clip_meta(at::TensorList grads, at::TensorList, int64_t, double) { return at::empty({}, grads[0].options().dtype(at::kFloat)); }
+
+template <typename F> c10::TypedOperatorHandle<F> handle(const char* name, F*) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").template typed<F>();
+}
+template <typename F, typename... Args> auto below_autograd(const c10::TypedOperatorHandle<F>& op, const Args&... args) {
+  const at::AutoDispatchBelowADInplaceOrView guard;
+  return op.call(args...);
+}
+
+// ---- what Python calls ------------------------------------------------------------------------------------------------
+
+variable_list call_forward(const Operands& o, int64_t plan, double factor, double eps, bool keep) {
+  static const auto op = handle("disco_amd::residual_norm_forward", &forward_op);
+  const auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+  return below_autograd(op, o.x, maybe(o.y), maybe(o.gate), maybe(o.scale), maybe(o.w1), maybe(o.b1), maybe(o.w2), maybe(o.b2), plan, factor, eps, keep);
+}
+
 class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
  public:
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1,
                                const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps) {
     const Plan p(plan);
     const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
-    Outputs r = ::forward(p, o, factor, eps, true);
+    variable_list outputs = call_forward(o, plan, factor, eps, true);
     ctx->set_materialize_grads(false);
     // without a next norm no gradient reads x: it is not kept, and may change
-    ctx->save_for_backward({p.pre ? o.x : Tensor(), o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, r.stats});
+    ctx->save_for_backward({p.pre ? o.x : Tensor(), o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, outputs.back()});
+    outputs.pop_back();
     ctx->saved_data["plan"] = plan;
     ctx->saved_data["floats"] = std::vector<double>{factor, eps};
-    variable_list outputs;
-    if (p.block) outputs.push_back(r.out);
-    if (p.pre) outputs.push_back(r.h);
     return outputs;
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = handle("disco_amd::residual_norm_backward", &backward_op);
     variable_list result(11);
+    const int64_t plan = ctx->saved_data["plan"].toInt();
     const auto floats = ctx->saved_data["floats"].toDoubleVector();
-    const Plan p(ctx->saved_data["plan"].toInt());
-    const Tensor dout = p.block ? rows(grads[0]) : Tensor(), dh = p.pre ? rows(grads[p.block ? 1 : 0]) : Tensor();
+    const Plan p(plan);
+    const Tensor dout = p.block ? grads[0] : Tensor(), dh = p.pre ? grads[p.block ? 1 : 0] : Tensor();
     if (!dout.defined() && !dh.defined()) return result;
     const variable_list s = ctx->get_saved_variables();
-    const Operands o{p.pre ? s[0] : dout, s[1], s[2], s[3], s[4], s[5], s[6], s[7]};      // dout: of x's shape and type
-    const c10::DeviceGuard guard(o.x.device());
-    const int64_t n = o.x.size(0), width = o.x.size(1);
     // without a gradient of h the stream's gradient is that of out itself
     const bool through = !dh.defined();
+    int64_t wanted = 0;
     for (size_t i = 0, edge = 0; i < 8; ++i) {      // edges are numbered over the operands that are there
       if ((i > 0 && !s[i].defined()) || !ctx->needs_input_grad(edge++)) continue;
       if (through && (i == 0 || i >= 6)) continue;
-      result[i] = at::empty(s[i].sizes(), s[i].options());
+      wanted |= (int64_t)1 << i;
     }
-    const size_t bytes = g_workspace(n, width);
-    const Tensor ws = at::empty({(int64_t)bytes}, o.x.options().dtype(at::kByte));
-    const disco_residual_norm d = describe(p, o, floats[0], floats[1]);
-    disco_residual_norm_grads g{};
-    g.dout = read(dout); g.dh = read(dh);
-    g.dx = write(result[0]); g.dy = write(result[1]); g.dgate = write(result[2]); g.dscale = write(result[3]);
-    g.dpost_weight = write(result[4]); g.dpost_bias = write(result[5]); g.dpre_weight = write(result[6]); g.dpre_bias = write(result[7]);
-    g.ld_dout = pitch(dout, width); g.ld_dh = pitch(dh, width); g.ld_dx = pitch(result[0], width); g.ld_dy = pitch(result[1], width);
-    g.ld_dgate = pitch(result[2], width);
-    // autograd makes the forward's stream current for its node, whichever one the caller of the backward is on
-    check(g_backward(&d, static_cast<const float*>(read(s[8])), &g, write(ws), bytes, stream_of(o.x.device())), "disco_residual_norm_backward");
+    if (wanted) {
+      const auto maybe = [](const Tensor& t) { return t.defined() ? Maybe(t) : Maybe(); };
+      const variable_list got = below_autograd(op, maybe(dout), maybe(dh), maybe(s[8]), maybe(s[0]), maybe(s[1]), maybe(s[2]), maybe(s[3]), maybe(s[4]),
+                                               maybe(s[5]), maybe(s[6]), maybe(s[7]), plan, floats[0], floats[1], wanted);
+      for (size_t i = 0, next = 0; i < 8; ++i)
+        if (wanted >> i & 1) result[i] = got[next++];
+    }
     if (through && ctx->needs_input_grad(0)) result[0] = dout;
     if (at::GradMode::is_enabled()) {      // the gradients have no formula of their own: whoever differentiates them is told
       for (Tensor& t : result)
@@ -174,9 +288,8 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
   }
 };
 
-std::vector<Tensor> residual_norm(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1,
-                                  const Maybe& w2, const Maybe& b2, int64_t plan, double factor, double eps, int64_t /*stream: unused*/) {
-  TORCH_CHECK(g_forward && g_backward && g_workspace && g_status, "disco_torch: not bound to libdisco_hip.so");
+variable_list residual_norm(const Tensor& x, const Maybe& y, const Maybe& gate, const Maybe& scale, const Maybe& w1, const Maybe& b1, const Maybe& w2,
+                            const Maybe& b2, int64_t plan, double factor, double eps, int64_t /*stream: unused*/) {
   const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
   bool grad = false;
   for (const Tensor* t : {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2}) {
@@ -184,14 +297,8 @@ std::vector<Tensor> residual_norm(const Tensor& x, const Maybe& y, const Maybe& 
     grad = grad || (t->defined() && t->requires_grad());
   }
   TORCH_CHECK(x.is_cuda(), "x is on ", x.device(), ": disco_amd runs on the GPU only, there is no CPU fallback");
-  grad = grad && at::GradMode::is_enabled();
-  if (grad) return ResidualNorm::apply(x, y, gate, scale, w1, b1, w2, b2, plan, factor, eps);
-  const Plan p(plan);
-  const Outputs r = forward(p, o, factor, eps, false);
-  std::vector<Tensor> outputs;
-  if (p.block) outputs.push_back(r.out);
-  if (p.pre) outputs.push_back(r.h);
-  return outputs;
+  if (grad && at::GradMode::is_enabled()) return ResidualNorm::apply(x, y, gate, scale, w1, b1, w2, b2, plan, factor, eps);
+  return call_forward(o, plan, factor, eps, false);
 }
 
 bool known(const Tensor& t) {
@@ -201,50 +308,30 @@ bool known(const Tensor& t) {
 
 // The norm over the gradients; with `out` also their clipping into it (out may be the list itself).  No value where the
 // tensors are not what the kernels read -- on one GPU, of a known type, without gaps, each output of its gradient's shape,
-// strides and type or float32, none sharing memory: gradients.py then says what is wrong, or makes copies.
+// strides and type or float32: gradients.py then says what is wrong, or makes copies.
 std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std::optional<std::vector<Tensor>>& out, int64_t norm_type, double max_norm,
                                     int64_t /*stream: unused*/) {
-  TORCH_CHECK(g_norm && g_clip && g_norm_workspace, "disco_torch: not bound to libdisco_hip.so");
   for (const Tensor& t : grads) refuse_tangent(t, "gradient_norm");
   if (out)
     for (const Tensor& t : *out) refuse_tangent(t, "gradient_norm");
   const size_t n = grads.size();
   if (n == 0 || !grads[0].is_cuda() || (out && out->size() != n)) return std::nullopt;
   const auto device = grads[0].device();
-  std::vector<const void*> src(n);
-  std::vector<void*> dst(out ? n : 0);
-  std::vector<int64_t> numel(n);
-  std::vector<int> type(n), out_type(out ? n : 0);
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
     if (g.layout() != at::kStrided || g.device() != device || !known(g) || (g.numel() > 0 && !g.is_non_overlapping_and_dense())) return std::nullopt;
-    src[i] = g.const_data_ptr();
-    numel[i] = g.numel();
-    type[i] = type_code(g);
-    if (!out) continue;
+    if (!out || (*out)[i].is_same(g)) continue;
     const Tensor& o = (*out)[i];
-    if (!o.is_same(g)) {
-      if (o.layout() != at::kStrided || o.device() != device || (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat) ||
-          o.sizes() != g.sizes() || (g.numel() > 0 && o.strides() != g.strides() && !(o.is_contiguous() && g.is_contiguous())))
-        return std::nullopt;
-    }
-    dst[i] = o.mutable_data_ptr();
-    out_type[i] = type_code(o);
+    if (o.layout() != at::kStrided || o.device() != device || (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat) ||
+        o.sizes() != g.sizes() || (g.numel() > 0 && o.strides() != g.strides() && !(o.is_contiguous() && g.is_contiguous())))
+      return std::nullopt;
   }
-  const c10::DeviceGuard guard(device);
-  const auto options = at::TensorOptions().device(device);
-  const size_t bytes = g_norm_workspace((int64_t)n);
-  const Tensor ws = at::empty({(int64_t)bytes}, options.dtype(at::kByte)), norm = at::empty({}, options.dtype(at::kFloat));
-  float* to = static_cast<float*>(norm.mutable_data_ptr());
   if (!out) {
-    check(g_norm(src.data(), numel.data(), type.data(), (int64_t)n, (int)norm_type, to, write(ws), bytes, stream_of(device)),
-          "disco_grad_norm");
-    return norm;
+    static const auto op = handle("disco_amd::grad_norm", &norm_op);
+    return below_autograd(op, at::TensorList(grads), norm_type);
   }
-  const int status = g_clip(src.data(), dst.data(), numel.data(), type.data(), out_type.data(), (int64_t)n, (int)norm_type, max_norm, to, write(ws),
-                            bytes, stream_of(device));
-  if (status == DISCO_EINVAL) return std::nullopt;
-  check(status, "disco_grad_clip");
+  static const auto op = handle("disco_amd::grad_clip", &clip_op);
+  const Tensor norm = below_autograd(op, at::TensorList(grads), at::TensorList(*out), norm_type, max_norm);
   for (const Tensor& o : *out)      // written behind autograd's back: whoever saved one of them must notice
     if (!o.is_inference()) torch::autograd::impl::bump_version(o);
   return norm;
@@ -260,4 +347,26 @@ TORCH_LIBRARY(disco_amd, m) {
       "residual_norm(Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? post_weight, Tensor? post_bias, Tensor? pre_weight, "
       "Tensor? pre_bias, int plan, float factor, float eps, int stream=0) -> Tensor[]",
       &residual_norm);
+  m.def(
+      "residual_norm_forward(Tensor x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? post_weight, Tensor? post_bias, Tensor? pre_weight, "
+      "Tensor? pre_bias, int plan, float factor, float eps, bool keep) -> Tensor[]");
+  m.def(
+      "residual_norm_backward(Tensor? dout, Tensor? dh, Tensor? stats, Tensor? x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? post_weight, "
+      "Tensor? post_bias, Tensor? pre_weight, Tensor? pre_bias, int plan, float factor, float eps, int wanted) -> Tensor[]");
+  m.def("grad_norm(Tensor[] grads, int norm_type) -> Tensor");
+  m.def("grad_clip(Tensor[] grads, Tensor(a!)[] out, int norm_type, float max_norm) -> Tensor");
+}
+
+TORCH_LIBRARY_IMPL(disco_amd, CUDA, m) {
+  m.impl("residual_norm_forward", &forward_op);
+  m.impl("residual_norm_backward", &backward_op);
+  m.impl("grad_norm", &norm_op);
+  m.impl("grad_clip", &clip_op);
+}
+
+TORCH_LIBRARY_IMPL(disco_amd, Meta, m) {
+  m.impl("residual_norm_forward", &forward_meta);
+  m.impl("residual_norm_backward", &backward_meta);
+  m.impl("grad_norm", &norm_meta);
+  m.impl("grad_clip", &clip_meta);
 }

@@ -262,3 +262,14 @@ def test_clipping_is_seen_by_autograd():
         check_norm(ops.clip_grads([h], 1.0), math.sqrt(10.0))
     want = norm64([h], 2)                        # max_norm * norm / (norm + 1e-6), not quite max_norm
     check_norm(ops.clip_grads([h, torch.zeros(3, device=DEV)], 5.0), want)
+
+
+def test_a_recorded_graph_clips():
+    from torch.fx.experimental.proxy_tensor import make_fx
+    grads = make([100, 3000], DTYPES[:1], seed=21)
+    graph = make_fx(lambda *g: (ops.grad_norm(g), ops.clip_grads(g, 0.5)))(*[g.clone() for g in grads])
+    other = [g * 2 for g in grads]
+    eager = [g.clone() for g in other]
+    n1, n2 = graph(*other)
+    want = ops.clip_grads(eager, 0.5)
+    assert torch.equal(n1, want) and torch.equal(n2, want) and all(torch.equal(a, b) for a, b in zip(other, eager))

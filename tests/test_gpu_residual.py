@@ -592,3 +592,65 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
     ops.row_norm(d), ops.row_norm(x, dw)      # outside of the level they are ordinary tensors
+
+
+@pytest.mark.parametrize("gate,pre", [("full", "layer"), ("row", "rms"), (None, None)])
+def test_a_recorded_graph_computes_the_same(gate, pre):
+    """make_fx records forward and backward; the graph gives the eager results, on other inputs too."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    s = make(20, 30, gate=gate, pre=pre, seed=81)
+    names = list(s["t"])
+
+    def step(*leaves):
+        out, h = call(s, dict(zip(names, leaves)))
+        return (out,) + (() if h is None else (h,)) + torch.autograd.grad([out] if h is None else [out, h], leaves,
+                                                                          [s["dout"]] if h is None else [s["dout"], s["dh"]])
+
+    leaves = [t.clone().requires_grad_() for t in s["t"].values()]
+    graph = make_fx(step)(*leaves)
+    targets = {n.target for n in graph.graph.nodes}
+    assert {torch.ops.disco_amd.residual_norm_forward.default, torch.ops.disco_amd.residual_norm_backward.default} <= targets
+    other = [torch.randn_like(t).requires_grad_() for t in leaves]
+    for a, b in zip(graph(*other), step(*other)):
+        assert torch.equal(a, b)
+
+
+def test_the_operators_pass_the_dispatchers_checks():
+    s = make(6, 20, "f32", "bf16", seed=82)
+    t = s["t"]
+    args = (t["x"], t["y"], t["gate"], t["scale"], t["post_weight"], t["post_bias"], t["pre_weight"], t["pre_bias"])
+    plan = 2 | 2 << 2 | 1 << 4 | 1 << 6 | 2 << 8 | 1 << 12
+    D = torch.ops.disco_amd
+    forward = (*args, plan, 1.0, EPS, True)
+    out, h, stats = D.residual_norm_forward(*forward)
+    want = call(s)
+    assert torch.equal(out, want[0]) and torch.equal(h, want[1]) and stats.shape == (24,)
+    backward = (s["dout"], s["dh"], stats, *args, plan, 1.0, EPS, 255)
+    for a, b in zip(D.residual_norm_backward(*backward), train(s)[2].values()):
+        assert torch.equal(a, b)
+    grads = [torch.randn(50, device=DEV), torch.randn(7, 3, device=DEV)]
+    for op, a in ((D.residual_norm_forward, forward), (D.residual_norm_backward, backward), (D.grad_norm, (grads, 2)),
+                  (D.grad_clip, (grads, [torch.empty_like(g) for g in grads], 2, 0.5))):
+        torch.library.opcheck(op.default, a, test_utils=("test_schema", "test_faketensor"))
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_a_compiled_function_computes_the_same(backend):
+    s = make(20, 30, seed=83)
+    names = list(s["t"])
+
+    def f(*leaves):
+        out, h = call(s, dict(zip(names, leaves)))
+        return out * s["dout"], h * s["dh"]
+
+    def step(g):
+        leaves = [t.clone().requires_grad_() for t in s["t"].values()]
+        return torch.autograd.grad([v.sum() for v in g(*leaves)], leaves)
+
+    try:
+        for a, b in zip(step(torch.compile(f, backend=backend)), step(f)):
+            assert torch.equal(a, b)
+        p, q = s["t"]["x"].clone(), s["t"]["x"].clone()
+        assert torch.equal(torch.compile(lambda t: ops.clip_grads([t], 0.5), backend=backend)(p), ops.clip_grads([q], 0.5)) and torch.equal(p, q)
+    finally:
+        torch._dynamo.reset()

@@ -209,3 +209,19 @@ def test_forward_mode_derivatives_are_refused():
         for grads, out in (([x, d], None), ([x, x], [d, x])):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 norm(grads, out, 2, 1.0)
+
+
+def test_a_trace_holds_the_operators():
+    """Fake tensors pass through, and a recorded graph holds the calls (not the empty buffers that they fill)."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    with FakeTensorMode():
+        x, y, w = torch.empty(6, 8, device="cuda"), torch.empty(6, 8, device="cuda", dtype=torch.bfloat16), torch.empty(8, device="cuda")
+        out, h = ops.residual_norm(x, y, post="rms", post_weight=w, pre="layer")
+        assert out.dtype == torch.float32 and h.dtype == torch.bfloat16 and out.shape == h.shape == (6, 8)
+        assert ops.grad_norm([x, y]).shape == ()
+        block = make_fx(lambda x, y, w: ops.residual_norm(x, y, post="rms", post_weight=w, pre="layer"))(x, y, w)
+        clip = make_fx(lambda x, w: (ops.grad_norm([x, w]), ops.clip_grads([x, w], 1.0), x))(x, w)
+    calls = [[n.target for n in g.graph.nodes if n.op == "call_function"] for g in (block, clip)]
+    assert torch.ops.disco_amd.residual_norm_forward.default in calls[0] and torch.ops.aten.empty.memory_format not in calls[0]
+    assert calls[1] == [torch.ops.disco_amd.grad_norm.default, torch.ops.disco_amd.grad_clip.default]
