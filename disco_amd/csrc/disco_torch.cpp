@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <memory>
 #include <optional>
@@ -301,6 +302,18 @@ variable_list residual_norm(const Tensor& x, const Maybe& y, const Maybe& gate, 
   return call_forward(o, plan, factor, eps, false);
 }
 
+// The norm has no derivative here.  Of gradients that are differentiated again it is a node that says so, not a constant.
+class GradientNorm : public torch::autograd::Function<GradientNorm> {
+ public:
+  static Tensor forward(AutogradContext*, at::TensorList grads, int64_t norm_type) {
+    static const auto op = handle("disco_amd::grad_norm", &norm_op);
+    return below_autograd(op, grads, norm_type);
+  }
+  static variable_list backward(AutogradContext*, variable_list) {
+    TORCH_CHECK(false, "grad_norm has no derivative: detach the gradients, or compute their norm with torch");
+  }
+};
+
 bool known(const Tensor& t) {
   const auto s = t.scalar_type();
   return s == at::kFloat || s == at::kHalf || s == at::kBFloat16;
@@ -327,8 +340,8 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
       return std::nullopt;
   }
   if (!out) {
-    static const auto op = handle("disco_amd::grad_norm", &norm_op);
-    return below_autograd(op, at::TensorList(grads), norm_type);
+    const bool grad = at::GradMode::is_enabled() && std::any_of(grads.begin(), grads.end(), [](const Tensor& g) { return g.requires_grad(); });
+    return grad ? GradientNorm::apply(at::TensorList(grads), norm_type) : GradientNorm::forward(nullptr, grads, norm_type);
   }
   static const auto op = handle("disco_amd::grad_clip", &clip_op);
   const Tensor norm = below_autograd(op, at::TensorList(grads), at::TensorList(*out), norm_type, max_norm);

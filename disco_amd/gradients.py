@@ -69,7 +69,7 @@ def _dense(g: torch.Tensor) -> bool:
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """``(sum |g|^p)^(1/p)`` over every element of every tensor, p = ``norm_type`` in {1, 2, inf}; a float32 scalar on the
     device.  Sums run in float64 in a fixed order: nothing overflows in between (a norm beyond float32 is infinite), and the
-    result does not vary."""
+    result does not vary.  It has no derivative: where a gradient requires one itself, differentiating the norm raises."""
     p = _norm_type(norm_type)
     grads = _list(grads)
     if not grads:
@@ -77,7 +77,7 @@ def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: flo
     norm = _launch(grads, None, p, 0.0)
     if norm is None:
         _check(grads)
-        norm = _launch([g.detach().contiguous() for g in grads], None, p, 0.0)
+        norm = _launch([g.contiguous() for g in grads], None, p, 0.0)
     return norm
 
 
@@ -88,7 +88,7 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     In place by default; ``out`` names one destination per gradient, of its shape and either its type or float32 (the
     buffers a mixed-precision optimiser reads).  Dense tensors that share memory are refused; views with gaps are read before
     anything is written, so that no element is scaled twice.  An infinite entry scales by zero and a NaN makes every
-    gradient NaN; with ``error_if_nonfinite`` a norm that is not finite in float32 raises RuntimeError and changes nothing
+    gradient NaN.  Autograd records none of it.  With ``error_if_nonfinite`` a norm that is not finite in float32 raises RuntimeError and changes nothing
     (this waits for the GPU)."""
     p = _norm_type(norm_type)
     max_norm = float(max_norm)
@@ -99,7 +99,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     if not grads and not dst:
         return grad_norm(grads, norm_type)
     if error_if_nonfinite:
-        norm = grad_norm(grads, norm_type)
+        with torch.no_grad():
+            norm = grad_norm(grads, norm_type)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"the norm of the gradients is {float(norm)}: they were not clipped")
     norm = _launch(grads, dst, p, max_norm) if grads else None

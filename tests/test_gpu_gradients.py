@@ -273,3 +273,25 @@ def test_a_recorded_graph_clips():
     n1, n2 = graph(*other)
     want = ops.clip_grads(eager, 0.5)
     assert torch.equal(n1, want) and torch.equal(n2, want) and all(torch.equal(a, b) for a, b in zip(other, eager))
+
+
+def test_the_norm_is_no_constant_of_a_graph():
+    """Gradients of gradients: the norm has no derivative, and whoever differentiates it is told; without that it is a number like
+    any other, and clipping leaves no trace in the graph."""
+    x = torch.randn(50, device=DEV, requires_grad=True)
+    (g,) = torch.autograd.grad(x.pow(3).sum(), x, create_graph=True)
+    norm = ops.grad_norm([g, torch.ones(3, device=DEV)])
+    check_norm(norm.detach(), norm64([g.detach(), torch.ones(3, device=DEV)], 2))
+    with pytest.raises(RuntimeError, match="no derivative"):
+        (norm * 2.0).backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(g.sum() + norm, x, retain_graph=True)
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(ops.grad_norm(torch.stack([g, g], 1)[:, 0]), x, retain_graph=True)      # a view with gaps
+    with pytest.raises(RuntimeError, match="no derivative"):
+        torch.autograd.grad(ops.grad_norm([x]), x)
+    with torch.no_grad():
+        assert not ops.grad_norm([g]).requires_grad
+    assert not ops.grad_norm([g.detach()]).requires_grad and not ops.clip_grads([g.detach().clone()], 1.0).requires_grad
+    (h,) = torch.autograd.grad(g.sum(), x)
+    assert torch.allclose(h, 6 * x.detach(), rtol=4 * U)
