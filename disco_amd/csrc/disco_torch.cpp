@@ -333,8 +333,10 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
     if (g.layout() != at::kStrided || g.device() != device || !known(g) || (g.numel() > 0 && !g.is_non_overlapping_and_dense())) return std::nullopt;
-    if (!out || (*out)[i].is_same(g)) continue;
+    if (!out) continue;
     const Tensor& o = (*out)[i];
+    if (g.is_neg() || o.is_neg()) return std::nullopt;      // negated when read: an operator that writes cannot take them
+    if (o.is_same(g)) continue;
     if (o.layout() != at::kStrided || o.device() != device || (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat) ||
         o.sizes() != g.sizes() || (g.numel() > 0 && o.strides() != g.strides() && !(o.is_contiguous() && g.is_contiguous())))
       return std::nullopt;

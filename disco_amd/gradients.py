@@ -56,6 +56,8 @@ def _launch(grads: Sequence[torch.Tensor], out, p: int, max_norm: float) -> Opti
 
 def _dense(g: torch.Tensor) -> bool:
     """Elements fill one block of memory, in any order of the dimensions: the kernels may walk it as it lies."""
+    if g.is_neg():
+        return False
     if g.is_contiguous():
         return True
     expected = 1
@@ -118,7 +120,7 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
             continue
         if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
             raise ValueError(_SHARED)
-        src.append(g.detach().contiguous())
+        src.append(g.detach().resolve_neg().contiguous())
         to.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
         back.append((o, to[-1]))
     norm = _launch(src, to, p, max_norm)

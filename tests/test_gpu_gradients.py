@@ -295,3 +295,23 @@ def test_the_norm_is_no_constant_of_a_graph():
     assert not ops.grad_norm([g.detach()]).requires_grad and not ops.clip_grads([g.detach().clone()], 1.0).requires_grad
     (h,) = torch.autograd.grad(g.sum(), x)
     assert torch.allclose(h, 6 * x.detach(), rtol=4 * U)
+
+
+def test_lazily_negated_gradients():
+    """Views that are negated when read (torch's negative bit): gradients and destinations, dense and with gaps."""
+    z = torch.randn(40, 2, device=DEV)
+    for view in (torch._neg_view, lambda t: torch._neg_view(t[:, :1])):
+        store = z.clone()
+        g = view(store)
+        assert g.is_neg()
+        keep = g.clone()
+        want = norm64([keep], 2)
+        check_norm(ops.grad_norm([g, torch.zeros(3, device=DEV)]), want)
+        to = torch.empty_like(keep)
+        check_norm(ops.clip_grads([g], 0.5, out=[to]), want)
+        check_clip([keep], [to], 0.5, want)
+        to = view(torch.zeros(40, 2, device=DEV))
+        check_norm(ops.clip_grads([keep], 0.5, out=[to]), want)
+        check_clip([keep], [to], 0.5, want)
+        check_norm(ops.clip_grads([g], 0.5), want)
+        check_clip([keep], [g], 0.5, want)

@@ -654,3 +654,34 @@ def test_a_compiled_function_computes_the_same(backend):
         assert torch.equal(torch.compile(lambda t: ops.clip_grads([t], 0.5), backend=backend)(p), ops.clip_grads([q], 0.5)) and torch.equal(p, q)
     finally:
         torch._dynamo.reset()
+
+
+def test_lazily_negated_operands():
+    """The imaginary part of a conjugate is negated when it is read: a row gate and a single column are passed as they lie."""
+    z = torch.randn(30, 1, device=DEV, dtype=torch.complex64)
+    v = z.conj().imag
+    assert v.is_neg()
+    s = make(30, 16, gate="row", seed=91)
+    s["t"]["gate"] = v.clone()
+    want = train(s)
+    s["t"]["gate"] = v
+    for a, b in zip(call(s), want):
+        assert torch.equal(a, b)
+    g = {k: t.requires_grad_() for k, t in s["t"].items() if k != "gate"}
+    out, h = call(s, {**g, "gate": z.requires_grad_().conj().imag})
+    got = torch.autograd.grad([out, h], list(g.values()) + [z], [s["dout"], s["dh"]])
+    for k, d in zip(g, got):
+        assert torch.equal(d, want[2][k]), k
+    assert torch.equal(got[-1].imag, -want[2]["gate"]) and not got[-1].real.any()
+    one = make(30, 1, gate=None, act=None, seed=92)
+    one["t"]["x"] = v.clone()
+    want = call(one)
+    one["t"]["x"] = v.detach()
+    for a, b in zip(call(one), want):
+        assert torch.equal(a, b)
+    n = torch._neg_view(torch.randn(7, 12, device=DEV))
+    assert torch.equal(ops.row_norm(n), ops.row_norm(n.clone()))
+    x = torch.randn(7, 12, device=DEV, requires_grad=True)
+    up = torch.randn(7, 12, device=DEV)
+    for a, b in zip(torch.autograd.grad(ops.row_norm(x), x, torch._neg_view(up)), torch.autograd.grad(ops.row_norm(x), x, -up)):
+        assert torch.equal(a, b)
