@@ -100,6 +100,7 @@ class JumpingKnowledge(torch.nn.Module):
 class BasicGNN(torch.nn.Module):
     supports_edge_weight = True
     supports_edge_attr = False
+    residual = False                                    # also of models pickled before there were residual blocks
 
     def __init__(self, nfeat: int, nhid: int, nlayers: int, nclass: Optional[int] = None, dropout: float = 0.0,
                  act: Union[str, Callable, None] = "relu", act_first: bool = False, act_kwargs: Optional[Dict[str, Any]] = None,

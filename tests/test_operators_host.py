@@ -225,3 +225,39 @@ def test_a_trace_holds_the_operators():
     calls = [[n.target for n in g.graph.nodes if n.op == "call_function"] for g in (block, clip)]
     assert torch.ops.disco_amd.residual_norm_forward.default in calls[0] and torch.ops.aten.empty.memory_format not in calls[0]
     assert calls[1] == [torch.ops.disco_amd.grad_norm.default, torch.ops.disco_amd.grad_clip.default]
+
+
+class _Dense(torch.nn.Module):
+    """Stands for a convolution where no graph is needed."""
+
+    def __init__(self, nfeat, nclass):
+        super().__init__()
+        self.lin = torch.nn.Linear(nfeat, nclass)
+
+    def reset_parameters(self):
+        self.lin.reset_parameters()
+
+    def forward(self, x, adj, edge_weight=None):
+        return self.lin(x)
+
+
+def test_models_from_before_residual_blocks_still_run():
+    """A model pickled whole when BasicGNN had no residual blocks has no such attribute."""
+    import copy
+    from collections import namedtuple
+    from disco_amd.models import basicgnn_large as M
+
+    class Net(M.BasicGNN):
+        def init_conv(self, nfeat, nclass, **kwargs):
+            return _Dense(nfeat, nclass)
+
+    new = Net(nfeat=6, nhid=8, nlayers=3, nclass=4).eval()
+    old = copy.deepcopy(new)
+    old.__dict__.pop("residual", None)
+    x = torch.randn(5, 6)
+    Batch = namedtuple("Batch", ["adj_t"])
+    adj = torch.zeros(1)
+    for call in (lambda m: m.forward(x, None), lambda m: m.forward_sampler(x, [(None, None, None)] * 3),
+                 lambda m: m.inference(x, [(5, torch.arange(5), Batch(adj))], "cpu")):
+        assert torch.equal(call(old), call(new))
+    old.initialize()
