@@ -13,8 +13,9 @@ On MI355X the graph stays resident: ``predict(x, adj)`` with a device-resident `
 and ``full_inference`` replaces the sampler round trips of ``large_inference`` by full-graph propagation.
 
 ``residual=True`` (or a dict of ``ResidualNorm`` arguments) makes every hidden layer behind the first a residual block: the
-first layer opens the stream, each further one reads its norm and is joined to it, the last reads the last norm.  Not in the
-reference; without it nothing changes.
+first layer opens the stream, each further one reads its norm and is joined to it, the last reads the last norm.  A block's
+activation comes in front of its norm, whatever ``act_first`` says (that orders the activation and ``norm``, which residual
+networks do not have).  Not in the reference; without it nothing changes.
 """
 from __future__ import annotations
 
@@ -105,9 +106,10 @@ class BasicGNN(torch.nn.Module):
     def __init__(self, nfeat: int, nhid: int, nlayers: int, nclass: Optional[int] = None, dropout: float = 0.0,
                  act: Union[str, Callable, None] = "relu", act_first: bool = False, act_kwargs: Optional[Dict[str, Any]] = None,
                  norm: Union[str, Callable, None] = None, norm_kwargs: Optional[Dict[str, Any]] = None,
-                 jk: Optional[str] = None, sgc: bool = False, residual: Union[bool, Dict[str, Any]] = False, **kwargs):
+                 jk: Optional[str] = None, sgc: bool = False, residual: Union[bool, Dict[str, Any], None] = False, **kwargs):
         super().__init__()
-        if residual is not False and (sgc or jk is not None or norm is not None or nclass is None or nlayers < 3):
+        self.residual = bool(residual) or isinstance(residual, dict)      # an empty dict: blocks with every default
+        if self.residual and (sgc or jk is not None or norm is not None or nclass is None or nlayers < 3):
             raise ValueError("residual blocks need three layers or more and an output width, and replace norm, jk and sgc")
         self.nfeat, self.nhid = nfeat, nhid
         self.temp_layers = nlayers                      # basicgnn_large.py:80-85: SGC is ONE conv with K = nlayers
@@ -145,9 +147,8 @@ class BasicGNN(torch.nn.Module):
             self.jk = JumpingKnowledge(jk, nhid, nlayers)
         if jk is not None:
             self.lin = Linear(nlayers * nhid if jk == "cat" else nhid, self.nclass)
-        self.residual = residual is not False
         if self.residual:
-            config = {} if residual is True else dict(residual)
+            config = {} if isinstance(residual, int) else dict(residual)      # True is an int
             self.joins = ModuleList(ResidualNorm(nhid, **config) for _ in range(nlayers - 2))
             self.first_norm = RowNorm(nhid, self.joins[0].pre.kind, self.joins[0].eps)
 

@@ -261,3 +261,14 @@ def test_models_from_before_residual_blocks_still_run():
                  lambda m: m.inference(x, [(5, torch.arange(5), Batch(adj))], "cpu")):
         assert torch.equal(call(old), call(new))
     old.initialize()
+
+
+@pytest.mark.parametrize("off", [False, None, 0])
+def test_residual_blocks_can_be_switched_off(off):
+    from disco_amd.models import basicgnn_large as M
+    for kw in (dict(nlayers=4), dict(nlayers=2, norm="BatchNorm"), dict(nlayers=3, jk="cat")):
+        m = M.GCN(nfeat=6, nhid=8, nclass=3, residual=off, **kw)
+        assert m.residual is False and not hasattr(m, "joins")
+    for on in (True, 1, {}, dict(pre="rms"), [("pre", "rms")]):
+        m = M.GCN(nfeat=6, nhid=8, nclass=3, nlayers=4, residual=on)
+        assert m.residual is True and len(m.joins) == 2
