@@ -1,7 +1,7 @@
 """Builds libdisco_hip.so (hand-written HIP kernels + C ABI) for gfx950 with hipcc.
 
 The library is built IN-TREE (``disco_amd/csrc/libdisco_hip.so``) so that the binary travels with
-the source tree to the GPU box; nothing is JIT-compiled at import time.
+the source tree; nothing is JIT-compiled at import time.
 """
 from __future__ import annotations
 
@@ -55,8 +55,6 @@ def build_torch_lib(force: bool = False) -> str:
 
 def build_lib(force: bool = False, extra_flags=(), name: str = "libdisco_hip.so", verbose: bool = False) -> str:
     out = lib_path(name)
-    if name == "libdisco_hip.so":
-        build_torch_lib(force)
     if not force and os.path.exists(out) and os.path.getmtime(out) >= _newest_source_mtime():
         return out
     hipcc = _hipcc()
@@ -93,5 +91,12 @@ def build_lib(force: bool = False, extra_flags=(), name: str = "libdisco_hip.so"
     return out
 
 
+def build_all(force: bool = False, verbose: bool = False) -> str:
+    """The C library, then the torch operators beside it (which need g++ and torch's headers).  Returns the C library's path."""
+    out = build_lib(force, verbose=verbose)
+    build_torch_lib(force)
+    return out
+
+
 if __name__ == "__main__":
-    print(build_lib(force="--force" in sys.argv, verbose=True))
+    print(build_all(force="--force" in sys.argv, verbose=True))

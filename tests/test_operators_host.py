@@ -272,3 +272,14 @@ def test_residual_blocks_can_be_switched_off(off):
     for on in (True, 1, {}, dict(pre="rms"), [("pre", "rms")]):
         m = M.GCN(nfeat=6, nhid=8, nclass=3, nlayers=4, residual=on)
         assert m.residual is True and len(m.joins) == 2
+
+
+def test_the_c_library_is_built_without_torch(monkeypatch):
+    """libdisco_hip.so needs hipcc alone; libdisco_torch.so is built beside it, after it."""
+    from disco_amd import build
+    called = []
+    monkeypatch.setattr(build, "build_torch_lib", lambda *a, **k: called.append("torch") or "")
+    monkeypatch.setattr(build, "_newest_source_mtime", lambda: 0.0)
+    assert build.build_lib() == build.lib_path() and called == []
+    monkeypatch.setattr(build, "build_lib", lambda *a, **k: called.append("hip") or "lib")
+    assert build.build_all() == "lib" and called == ["hip", "torch"]
