@@ -9,6 +9,7 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
@@ -18,6 +19,7 @@
 #include <cstdint>
 #include <memory>
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "../../include/disco_hip.h"
@@ -201,6 +203,8 @@ struct List {
   }
 };
 
+constexpr const char* kShared = "clip_grads: two tensors share memory; each gradient may be scaled only once";
+
 Tensor norm_op(at::TensorList grads, int64_t norm_type) {
   const c10::DeviceGuard guard(grads[0].device());
   const List l(grads, nullptr);
@@ -214,7 +218,7 @@ Tensor clip_op(at::TensorList grads, at::TensorList out, int64_t norm_type, doub
   const List l(grads, &out);
   const int status = g_clip(l.src.data(), l.dst.data(), l.numel.data(), l.type.data(), l.out_type.data(), (int64_t)grads.size(), (int)norm_type, max_norm,
                             static_cast<float*>(write(l.norm)), write(l.ws), (size_t)l.ws.numel(), stream_of(grads[0].device()));
-  TORCH_CHECK_VALUE(status != DISCO_EINVAL, "clip_grads: two tensors share memory; each gradient may be scaled only once");
+  TORCH_CHECK_VALUE(status != DISCO_EINVAL, kShared);
   check(status, "disco_grad_clip");
   return l.norm;
 }
@@ -319,6 +323,14 @@ bool known(const Tensor& t) {
   return s == at::kFloat || s == at::kHalf || s == at::kBFloat16;
 }
 
+// A gradient without gaps, in any order of its dimensions, and its destination (itself or another tensor) in the same order:
+// the kernels may walk the pair as it lies.
+bool walkable(const Tensor& g, const Tensor& o) {
+  if (g.is_neg() || o.is_neg()) return false;      // negated when read: an operator that writes cannot take them
+  if (g.numel() == 0) return true;
+  return g.is_non_overlapping_and_dense() && (o.is_same(g) || o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous()));
+}
+
 // The norm over the gradients; with `out` also their clipping into it (out may be the list itself).  No value where the
 // tensors are not what the kernels read -- on one GPU, of a known type, without gaps, each output of its gradient's shape,
 // strides and type or float32: gradients.py then says what is wrong, or makes copies.
@@ -335,11 +347,10 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
     if (g.layout() != at::kStrided || g.device() != device || !known(g) || (g.numel() > 0 && !g.is_non_overlapping_and_dense())) return std::nullopt;
     if (!out) continue;
     const Tensor& o = (*out)[i];
-    if (g.is_neg() || o.is_neg()) return std::nullopt;      // negated when read: an operator that writes cannot take them
-    if (o.is_same(g)) continue;
-    if (o.layout() != at::kStrided || o.device() != device || (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat) ||
-        o.sizes() != g.sizes() || (g.numel() > 0 && o.strides() != g.strides() && !(o.is_contiguous() && g.is_contiguous())))
+    if (!o.is_same(g) && (o.layout() != at::kStrided || o.device() != device || (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat) ||
+                          o.sizes() != g.sizes()))
       return std::nullopt;
+    if (!walkable(g, o)) return std::nullopt;
   }
   if (!out) {
     const bool grad = at::GradMode::is_enabled() && std::any_of(grads.begin(), grads.end(), [](const Tensor& g) { return g.requires_grad(); });
@@ -350,6 +361,99 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
   for (const Tensor& o : *out)      // written behind autograd's back: whoever saved one of them must notice
     if (!o.is_inference()) torch::autograd::impl::bump_version(o);
   return norm;
+}
+
+// Places of a view in memory: the bytes at + sum of stride_k * x_k + u, 0 <= x_k <= most_k, with u inside an element; the
+// strides fall and end with u's 1.
+struct Term { int64_t stride, most; };
+struct Places {
+  int64_t at, last;      // last byte
+  c10::SmallVector<Term, 6> terms;
+  Places(int64_t at_, c10::IntArrayRef size, c10::IntArrayRef stride, int64_t item) : at(at_), last(at_ + item - 1) {
+    for (size_t d = 0; d < size.size(); ++d)
+      if (size[d] > 1 && stride[d] > 0) {
+        terms.push_back({stride[d] * item, size[d] - 1});
+        last += terms.back().stride * terms.back().most;
+      }
+    std::sort(terms.begin(), terms.end(), [](const Term& p, const Term& q) { return p.stride > q.stride; });
+    terms.push_back({1, item - 1});
+  }
+};
+Places places(const Tensor& t) { return {(int64_t)reinterpret_cast<uintptr_t>(t.const_data_ptr()), t.sizes(), t.strides(), (int64_t)t.element_size()}; }
+
+// A sum of the terms from k on that is `target`; strides fall and end with 1.  After `work` steps the answer is yes: views that
+// nobody can tell apart are not told apart here.
+bool reaches(c10::ArrayRef<Term> terms, c10::ArrayRef<int64_t> rest, size_t k, int64_t target, int64_t& work) {
+  if (target < 0 || target > rest[k]) return false;
+  if (k + 1 == terms.size()) return true;
+  const int64_t s = terms[k].stride;
+  for (int64_t x = std::min(terms[k].most, target / s); x >= 0 && target - x * s <= rest[k + 1]; --x)
+    if (--work < 0 || reaches(terms, rest, k + 1, target - x * s, work)) return true;
+  return false;
+}
+
+// Whether two views have a byte in common.  With b's indices counted from their ends, a place of each is one sum of terms:
+// sum_a + sum_b' = (b's last byte) - (a's first).
+bool meet(const Places& a, const Places& b) {
+  if (a.last < b.at || b.last < a.at) return false;
+  c10::SmallVector<Term, 12> terms;
+  for (size_t i = 0, j = 0; i < a.terms.size() || j < b.terms.size();) {
+    const bool first = j == b.terms.size() || (i < a.terms.size() && a.terms[i].stride >= b.terms[j].stride);
+    const Term& t = first ? a.terms[i++] : b.terms[j++];
+    if (!terms.empty() && terms.back().stride == t.stride) terms.back().most += t.most;
+    else terms.push_back(t);
+  }
+  c10::SmallVector<int64_t, 12> rest(terms.size());
+  int64_t sum = 0;
+  for (size_t k = terms.size(); k-- > 0;) rest[k] = sum += terms[k].stride * terms[k].most;
+  int64_t work = 100000;
+  return reaches(terms, rest, 0, b.last - a.at, work);
+}
+
+// Two elements of one view at the same place: their indices differ first in some dimension d, and there it is enough to set
+// index 0 against the others.
+bool meets_itself(const Tensor& t) {
+  const int64_t item = (int64_t)t.element_size(), at = (int64_t)reinterpret_cast<uintptr_t>(t.const_data_ptr());
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) == 1) continue;
+    c10::SmallVector<int64_t, 6> size(t.sizes().begin() + d, t.sizes().end());
+    const auto stride = t.strides().slice(d);
+    size[0] = 1;
+    const Places first(at, size, stride, item);
+    size[0] = t.size(d) - 1;
+    if (meet(first, Places(at + stride[0] * item, size, stride, item))) return true;
+  }
+  return false;
+}
+
+// Whether an element would be written with two values: by two gradients, or by one into a view that meets itself.  Gradients
+// that are scaled where they lie may meet, since each writes what the other writes.
+bool written_twice(const std::vector<Tensor>& grads, const std::vector<Tensor>& out) {
+  std::vector<std::pair<Places, bool>> all;
+  for (size_t i = 0; i < out.size(); ++i) {
+    if (out[i].numel() == 0 || out[i].key_set().has(c10::DispatchKey::Python)) continue;      // a fake tensor has no memory
+    const bool in_place = out[i].is_same(grads[i]);
+    if (!in_place && !out[i].is_non_overlapping_and_dense() && meets_itself(out[i])) return true;
+    all.emplace_back(places(out[i]), in_place);
+  }
+  std::sort(all.begin(), all.end(), [](const auto& a, const auto& b) { return a.first.at < b.first.at; });
+  for (size_t i = 0; i < all.size(); ++i)
+    for (size_t j = i + 1; j < all.size() && all[j].first.at <= all[i].first.last; ++j)
+      if (!(all[i].second && all[j].second) && meet(all[i].first, all[j].first)) return true;
+  return false;
+}
+
+// Which pairs go through contiguous copies, because the kernels cannot walk them as they lie.
+std::vector<int64_t> copied_pairs(const std::vector<Tensor>& grads, const std::vector<Tensor>& out) {
+  TORCH_CHECK(grads.size() == out.size(), "copied_pairs: a destination for each gradient");
+  std::vector<int64_t> r;
+  bool in_place = true;
+  for (size_t i = 0; i < out.size(); ++i) {
+    in_place = in_place && out[i].is_same(grads[i]);
+    if (!walkable(grads[i], out[i])) r.push_back((int64_t)i);
+  }
+  TORCH_CHECK_VALUE(in_place || !written_twice(grads, out), kShared);
+  return r;
 }
 
 }  // namespace
@@ -368,6 +472,7 @@ TORCH_LIBRARY(disco_amd, m) {
   m.def(
       "residual_norm_backward(Tensor? dout, Tensor? dh, Tensor? stats, Tensor? x, Tensor? y, Tensor? gate, Tensor? scale, Tensor? post_weight, "
       "Tensor? post_bias, Tensor? pre_weight, Tensor? pre_bias, int plan, float factor, float eps, int wanted) -> Tensor[]");
+  m.def("copied_pairs(Tensor[] grads, Tensor[] out) -> int[]", &copied_pairs);
   m.def("grad_norm(Tensor[] grads, int norm_type) -> Tensor");
   m.def("grad_clip(Tensor[] grads, Tensor(a!)[] out, int norm_type, float max_norm) -> Tensor");
 }

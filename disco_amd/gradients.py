@@ -54,20 +54,6 @@ def _launch(grads: Sequence[torch.Tensor], out, p: int, max_norm: float) -> Opti
     return _lib.torch_op("gradient_norm")(grads, out, p, max_norm)
 
 
-def _dense(g: torch.Tensor) -> bool:
-    """Elements fill one block of memory, in any order of the dimensions: the kernels may walk it as it lies."""
-    if g.is_neg():
-        return False
-    if g.is_contiguous():
-        return True
-    expected = 1
-    for size, stride in sorted(((n, s) for n, s in zip(g.shape, g.stride()) if n > 1), key=lambda d: d[1]):
-        if stride != expected:
-            return False
-        expected *= size
-    return True
-
-
 def grad_norm(grads: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """``(sum |g|^p)^(1/p)`` over every element of every tensor, p = ``norm_type`` in {1, 2, inf}; a float32 scalar on the
     device.  Sums run in float64 in a fixed order: nothing overflows in between (a norm beyond float32 is infinite), and the
@@ -88,8 +74,8 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
     """Scales every gradient by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before (float32, on the device).
 
     In place by default; ``out`` names one destination per gradient, of its shape and either its type or float32 (the
-    buffers a mixed-precision optimiser reads).  Dense tensors that share memory are refused; views with gaps are read before
-    anything is written, so that no element is scaled twice.  An infinite entry scales by zero and a NaN makes every
+    buffers a mixed-precision optimiser reads).  Destinations that share memory are refused; views with gaps that are scaled
+    where they lie may share it: all are read before anything is written, so that no element is scaled twice.  An infinite entry scales by zero and a NaN makes every
     gradient NaN.  Autograd records none of it.  With ``error_if_nonfinite`` a norm that is not finite in float32 raises RuntimeError and changes nothing
     (this waits for the GPU)."""
     p = _norm_type(norm_type)
@@ -112,17 +98,14 @@ def clip_grads(grads: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: flo
         raise ValueError(f"out has {len(dst)} tensors for {len(grads)} gradients")
     _check(grads, dst)
     # the kernels walk memory in order: a pair that lies differently, or with gaps, goes through contiguous copies
-    src, to, back = [], [], []
-    for g, o in zip(grads, dst):
-        if _dense(o) and (o is g or (_dense(g) and o.stride() == g.stride())):
-            src.append(g)
-            to.append(o)
-            continue
+    src, to, back = list(grads), list(dst), []
+    for i in _lib.torch_op("copied_pairs")(grads, dst):
+        g, o = grads[i], dst[i]
         if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
             raise ValueError(_SHARED)
-        src.append(g.detach().resolve_neg().contiguous())
-        to.append(torch.empty(o.shape, dtype=o.dtype, device=o.device))
-        back.append((o, to[-1]))
+        src[i] = g.detach().resolve_neg().contiguous()
+        to[i] = torch.empty(o.shape, dtype=o.dtype, device=o.device)
+        back.append((o, to[i]))
     norm = _launch(src, to, p, max_norm)
     if norm is None:
         raise ValueError(_SHARED)

@@ -315,3 +315,25 @@ def test_lazily_negated_gradients():
         check_clip([keep], [to], 0.5, want)
         check_norm(ops.clip_grads([g], 0.5), want)
         check_clip([keep], [g], 0.5, want)
+
+
+def test_two_gradients_into_one_view_with_gaps_are_refused():
+    grads = make([(60, 48), (60, 48)], DTYPES[:1], seed=31)
+    hole = torch.full((60, 100), 5.0, device=DEV)
+    for out in ([hole[:, :48], hole[:, :48]], [hole[:, :48], hole[:, 47:95]], [hole[:, :48], hole.view(-1)[:60 * 49].view(60, 49)[:, :48]],
+                [grads[1][:, :48], grads[1]]):
+        before = [g.clone() for g in grads]
+        with pytest.raises(ValueError, match="share memory"):
+            ops.clip_grads(grads, 0.5, out=out)
+        assert (hole == 5).all() and all(torch.equal(a, b) for a, b in zip(grads, before))
+    out = [hole[:, :48], hole[:, 48:96]]                              # beside each other in one buffer
+    want = norm64(grads, 2)
+    check_norm(ops.clip_grads(grads, 0.5, out=out), want)
+    check_clip(grads, out, 0.5, want)
+    assert (hole[:, 96:] == 5).all()
+    wide = torch.randn(60, 100, device=DEV)                           # in place beside a destination of its own
+    keep = wide[:, :48].clone()
+    pair = [wide[:, :48], grads[1]]
+    want = norm64(pair, 2)
+    check_norm(ops.clip_grads(pair, 0.5, out=[pair[0], wide[:, 50:98]]), want)
+    check_clip([keep, grads[1]], [wide[:, :48], wide[:, 50:98]], 0.5, want)

@@ -283,3 +283,53 @@ def test_the_c_library_is_built_without_torch(monkeypatch):
     assert build.build_lib() == build.lib_path() and called == []
     monkeypatch.setattr(build, "build_lib", lambda *a, **k: called.append("hip") or "lib")
     assert build.build_all() == "lib" and called == ["hip", "torch"]
+
+
+def _written_twice(dst, in_place):
+    """Whether clipping refuses the destinations; those numbered in ``in_place`` are their gradients themselves."""
+    try:
+        _lib.torch_op("copied_pairs")([d if i in in_place else torch.empty(d.shape) for i, d in enumerate(dst)], dst)
+    except ValueError as e:
+        assert "share memory" in str(e)
+        return True
+    return False
+
+
+def test_destinations_that_would_be_written_twice():
+    t = torch.zeros(64, 100)
+    half = t.view(torch.float16)
+    same = t.as_strided((4, 4), (1, 1))
+    apart = t.as_strided((3, 2), (2, 3))          # 0 3 2 5 4 7
+    for dst, twice in (([t[:, :48], t[:, 48:]], False), ([t[:, :49], t[:, 48:]], True), ([t[:, ::2], t[:, 1::2]], False), ([t[:, ::2], t[:, ::4]], True),
+                       ([t, t[:, ::2]], True), ([t[:32], t[32:, ::2]], False), ([t[:, 3], t[:, 4]], False), ([t[::2, 3], t[4, ::3]], True),
+                       ([t[::2, 3], t[5, ::3]], False), ([same], True), ([apart], False), ([t.t()[:, ::2], t[1::2]], False), ([t[0:1].expand(5, 100)], True),
+                       ([t[:, :50], half[:, 100:]], False), ([t[:, :51], half[:, 100::2]], True), ([t[:0], t[:0]], False), ([t[0, 0], t[:, 1::2]], False),
+                       ([t[0, 1], t[:, 1::2]], True)):
+        for order in (dst, dst[::-1]):
+            assert _written_twice(order, ()) == twice, [(d.shape, d.stride(), d.storage_offset()) for d in order]
+            assert not _written_twice(order, range(len(dst)))
+            if len(dst) == 2:
+                assert _written_twice(order, (0,)) == twice
+
+
+def test_shared_memory_against_counting():
+    """Random views of a small buffer against the places that each of them really has."""
+    import random
+    r, base, met = random.Random(5), torch.zeros(400), 0
+
+    def view():
+        dims = r.randint(0, 3)
+        size, stride = [r.randint(1, 5) for _ in range(dims)], [r.choice([0, 1, 2, 3, 5, 7, 10, 20, 21]) for _ in range(dims)]
+        return base.as_strided(size, stride, r.randint(0, 60))
+
+    def places(v):
+        return [int(i) for i in torch.arange(400).as_strided(v.size(), v.stride(), v.storage_offset()).reshape(-1)]
+
+    for _ in range(3000):
+        a, b = view(), view()
+        p, q = places(a), places(b)
+        want = len(set(p)) < len(p) or len(set(q)) < len(q) or bool(set(p) & set(q))
+        assert _written_twice([a, b], ()) == want, (a.shape, a.stride(), a.storage_offset(), b.shape, b.stride(), b.storage_offset())
+        assert _written_twice([a, b], (0,)) == (len(set(q)) < len(q) or bool(set(p) & set(q)))
+        met += want
+    assert 500 < met < 2500
