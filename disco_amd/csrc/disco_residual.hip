@@ -201,6 +201,8 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
   if ((g->dpost_weight && !d->post_weight) || (g->dpost_bias && !d->post_bias) || (g->dpre_weight && !d->pre_weight) ||
       (g->dpre_bias && !d->pre_bias) || (g->dscale && !d->scale_vector) || (g->dgate && !d->gate_kind) || (g->dh && !d->pre_norm))
     return DISCO_EINVAL;
+  // out = x + scale * y: the gradient of y is that of out, scaled
+  const bool reads_y = d->post_norm || d->gate_kind || d->scale_vector || g->dh;
   ResidualArgs a;
   fill(d, &a);
   const bool channel = d->gate_kind == DISCO_GATE_CHANNEL;
@@ -212,7 +214,7 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
         (d->gate_kind == DISCO_GATE_ROW && g->dgate && g->ld_dgate < 1 && n > 1))
       return DISCO_EINVAL;
     if (d->ldx < 0 || d->ldy < 0 || d->ld_gate < 0 || g->ld_dout < 0 || g->ld_dh < 0) return DISCO_EINVAL;
-    if ((d->has_block && !d->y) || (g->dh && !d->x) || (d->gate_kind && !d->gate) || ((d->post_norm || g->dh) && !stats)) return DISCO_EINVAL;
+    if ((d->has_block && !d->y && (reads_y || !g->dout)) || (g->dh && !d->x) || (d->gate_kind && !d->gate) || ((d->post_norm || g->dh) && !stats)) return DISCO_EINVAL;
   }
   const ResidualShape s = residual_shape(F, d->block_type != DISCO_F32);
   const unsigned grid = backward_grid(n, s, residual_mode(d->has_block, d->gate_kind));
@@ -223,6 +225,10 @@ extern "C" int disco_residual_norm_backward(const disco_residual_norm* d, const 
   if (a.partials && summed > 0 && (!workspace || workspace_bytes < need)) return DISCO_EWORKSPACE;
   hipStream_t stream = static_cast<hipStream_t>(stream_);
   a.stats = const_cast<float*>(stats);
+  if (d->has_block && !a.y) {      // a row that is there, in place of one whose values go nowhere
+    a.y = g->dout;
+    a.ldy = 0;
+  }
   a.dout = g->dout; a.lddo = g->ld_dout; a.dh = g->dh; a.lddh = g->ld_dh;
   a.dx = g->dx; a.lddx = g->ld_dx; a.dy = g->dy; a.lddy = g->ld_dy; a.dg = channel ? nullptr : g->dgate; a.lddg = g->ld_dgate;
   a.partial = a.partials ? static_cast<float*>(workspace) : nullptr;

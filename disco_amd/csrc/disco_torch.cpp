@@ -139,11 +139,13 @@ Tensor rows(const Tensor& t) {
 }
 
 // The operands' gradients that `wanted` names (a bit for each operand, in the operator's order), in that order.
-variable_list backward_outputs(const Operands& o, int64_t wanted) {
+variable_list backward_outputs(const Plan& p, const Operands& o, int64_t wanted) {
   variable_list r;
   const Tensor* all[] = {&o.x, &o.y, &o.gate, &o.scale, &o.w1, &o.b1, &o.w2, &o.b2};
-  for (int i = 0; i < 8; ++i)
-    if (wanted >> i & 1) r.push_back(at::empty_symint(all[i]->sym_sizes(), all[i]->options()));
+  for (int i = 0; i < 8; ++i) {
+    const Tensor& t = all[i]->defined() ? *all[i] : o.x;      // y, where it was not kept
+    if (wanted >> i & 1) r.push_back(at::empty_symint(t.sym_sizes(), i == 1 ? t.options().dtype(type_of(p.block_type)) : t.options()));
+  }
   return r;
 }
 
@@ -155,7 +157,7 @@ variable_list backward_op(const Maybe& dout_, const Maybe& dh_, const Maybe& sta
   const Operands o = operands(x.value_or(dout), y, gate, scale, w1, b1, w2, b2);      // dout: of x's shape and type
   const c10::DeviceGuard guard(o.x.device());
   const int64_t n = o.x.size(0), width = o.x.size(1);
-  variable_list r = backward_outputs(o, wanted);
+  variable_list r = backward_outputs(p, o, wanted);
   size_t next = 0;
   const auto gradient = [&](int i) { return wanted >> i & 1 ? r[next++] : Tensor(); };
   const Tensor dx = gradient(0), dy = gradient(1), dgate = gradient(2), dscale = gradient(3), dw1 = gradient(4), db1 = gradient(5), dw2 = gradient(6),
@@ -175,8 +177,8 @@ variable_list backward_op(const Maybe& dout_, const Maybe& dh_, const Maybe& sta
 }
 
 variable_list backward_meta(const Maybe& dout, const Maybe&, const Maybe&, const Maybe& x, const Maybe& y, const Maybe& gate, const Maybe& scale,
-                            const Maybe& w1, const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t, double, double, int64_t wanted) {
-  return backward_outputs(operands(x.has_value() ? *x : *dout, y, gate, scale, w1, b1, w2, b2), wanted);
+                            const Maybe& w1, const Maybe& b1, const Maybe& w2, const Maybe& b2, int64_t plan, double, double, int64_t wanted) {
+  return backward_outputs(Plan(plan), operands(x.has_value() ? *x : *dout, y, gate, scale, w1, b1, w2, b2), wanted);
 }
 
 // The tensors of a list as the C entries take them.
@@ -250,8 +252,9 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Operands o = operands(x, y, gate, scale, w1, b1, w2, b2);
     variable_list outputs = call_forward(o, plan, factor, eps, true);
     ctx->set_materialize_grads(false);
-    // without a next norm no gradient reads x: it is not kept, and may change
-    ctx->save_for_backward({p.pre ? o.x : Tensor(), o.y, o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, outputs.back()});
+    // what no gradient reads is not kept, and may change: x without a next norm, y in out = x + factor * y
+    const bool reads_y = p.post || p.pre || p.gate || o.scale.defined();
+    ctx->save_for_backward({p.pre ? o.x : Tensor(), reads_y ? o.y : Tensor(), o.gate, o.scale, o.w1, o.b1, o.w2, o.b2, outputs.back()});
     outputs.pop_back();
     ctx->saved_data["plan"] = plan;
     ctx->saved_data["floats"] = std::vector<double>{factor, eps};
@@ -267,11 +270,12 @@ class ResidualNorm : public torch::autograd::Function<ResidualNorm> {
     const Tensor dout = p.block ? grads[0] : Tensor(), dh = p.pre ? grads[p.block ? 1 : 0] : Tensor();
     if (!dout.defined() && !dh.defined()) return result;
     const variable_list s = ctx->get_saved_variables();
+    const auto present = [&](size_t i) { return i == 0 || (i == 1 ? p.block : s[i].defined()); };
     // without a gradient of h the stream's gradient is that of out itself
     const bool through = !dh.defined();
     int64_t wanted = 0;
     for (size_t i = 0, edge = 0; i < 8; ++i) {      // edges are numbered over the operands that are there
-      if ((i > 0 && !s[i].defined()) || !ctx->needs_input_grad(edge++)) continue;
+      if (!present(i) || !ctx->needs_input_grad(edge++)) continue;
       if (through && (i == 0 || i >= 6)) continue;
       wanted |= (int64_t)1 << i;
     }

@@ -398,8 +398,8 @@ typedef struct disco_residual_norm_grads {
 } disco_residual_norm_grads;
 
 /* `stats` (float32 [4 * rows], may be NULL where no backward follows) keeps the rows' means and inverse deviations.  The
- * backward takes the forward's descriptor and stats, reads x (where dh is given), y and gate again and sums the vectors'
- * gradients in a fixed order through `workspace`.  Widths above DISCO_RESIDUAL_MAX_WIDTH: DISCO_EUNSUPPORTED. */
+ * backward takes the forward's descriptor and stats, reads x (where dh is given), y (where a norm, a gate, a scale vector or
+ * dh is given; NULL is allowed otherwise) and gate again and sums the vectors' gradients in a fixed order through `workspace`.  Widths above DISCO_RESIDUAL_MAX_WIDTH: DISCO_EUNSUPPORTED. */
 int disco_residual_norm_forward(const disco_residual_norm* desc_host, void* out, int64_t ld_out, void* h, int64_t ld_h,
                                 float* stats, void* stream);
 size_t disco_residual_norm_workspace_bytes(int64_t rows, int64_t width);

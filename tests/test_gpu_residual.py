@@ -685,3 +685,25 @@ def test_lazily_negated_operands():
     up = torch.randn(7, 12, device=DEV)
     for a, b in zip(torch.autograd.grad(ops.row_norm(x), x, torch._neg_view(up)), torch.autograd.grad(ops.row_norm(x), x, -up)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("stream,block", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f32", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("n,F", [(1, 1), (20, 30), (3, 4099), (40, 3), (2, 16384)])
+def test_the_blocks_output_may_change_where_no_gradient_reads_it(stream, block, n, F):
+    """out = x + factor * y: neither x nor y is kept."""
+    x, y = (torch.randn(n, F, device=DEV).to(T[k]).requires_grad_() for k in (stream, block))
+    up = torch.randn(n, F, device=DEV).to(T[stream])
+    a, b = x * 1.0, y * 1.0
+    out = ops.residual_norm(a, b, scale=0.3)
+    a.detach().fill_(float("nan"))
+    b.detach().fill_(float("nan"))
+    gx, gy = torch.autograd.grad(out, (x, y), up, retain_graph=True)
+    assert torch.equal(gx, up) and gy.dtype == T[block] and torch.equal(gy, (up.float() * 0.3).to(T[block]))
+    (gy,) = torch.autograd.grad(out, (y,), torch.full((1, 1), float("nan"), device=DEV, dtype=T[stream]).expand(n, F))
+    assert gy.isnan().all()
+    for kw in (dict(post="rms"), dict(gate=torch.ones(F, device=DEV)), dict(scale=torch.ones(F, device=DEV)), dict(pre="rms")):
+        b = y * 1.0
+        out = ops.residual_norm(x, b, **kw)
+        b.detach().add_(1.0)
+        with pytest.raises(RuntimeError, match="modified"):
+            sum(o.sum() for o in (out if isinstance(out, tuple) else (out,))).backward()

@@ -333,3 +333,13 @@ def test_shared_memory_against_counting():
         assert _written_twice([a, b], (0,)) == (len(set(q)) < len(q) or bool(set(p) & set(q)))
         met += want
     assert 500 < met < 2500
+
+
+def test_the_backward_asks_for_y_where_it_reads_it():
+    lib, G = _lib.load(), _lib.ResidualNormGrads
+    g = dict(dout=64, ld_dout=8, ld_dx=8, ld_dy=8, ld_dgate=8)      # nothing is wanted: nothing is launched
+    assert lib.disco_residual_norm_backward(_desc(y=None), None, G(**g), None, 0, None) == 0
+    for d, more in ((dict(post_norm=1), {}), (dict(gate_kind=1, gate=64), {}), (dict(gate_kind=3, gate=64), {}), (dict(scale_vector=64), {}),
+                    (dict(pre_norm=1), dict(dh=64, ld_dh=8)), ({}, dict(dout=None))):
+        assert lib.disco_residual_norm_backward(_desc(y=None, **d), 64, G(**{**g, **more}), None, 0, None) == -1
+        assert lib.disco_residual_norm_backward(_desc(**d), 64, G(**{**g, **more}), None, 0, None) == 0
