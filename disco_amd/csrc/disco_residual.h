@@ -87,10 +87,22 @@ __device__ __forceinline__ float activate(float g, int act) {
   if (act == DISCO_ACT_TANH) return tanhf(g);
   return g;
 }
-// derivative from the activation's own value
-__device__ __forceinline__ float activate_slope(float a, int act) {
-  if (act == DISCO_ACT_SIGMOID) return a * (1.0f - a);
-  if (act == DISCO_ACT_TANH) return 1.0f - a * a;
+// A gate as the backward keeps it: in one register, from which the activation a and its slope both come without cancellation.
+// Sigmoid: the smaller of a and 1 - a, which is e / (1 + e) with e = exp(-|g|), its sign bit set where a is the larger; the
+// slope is their product.  (From a alone, 1 - a has lost 4 digits at g = 8 and everything at 18.)  Tanh keeps its value, and
+// 1 - a * a what that leaves, as torch's does.
+__device__ __forceinline__ float gate_code(float g, int act) {
+  if (act == DISCO_ACT_SIGMOID) {
+    const float e = expf(-fabsf(g));
+    return __uint_as_float(__float_as_uint(-e * __builtin_amdgcn_rcpf(1.0f + e)) ^ (__float_as_uint(g) & 0x80000000u));
+  }
+  return act == DISCO_ACT_TANH ? tanhf(g) : g;
+}
+// `one`: the bits of 1.0 for a sigmoid, 0 otherwise
+__device__ __forceinline__ float gate_value(float c, int one) { return c + __int_as_float((__float_as_int(c) >> 31) & one); }
+__device__ __forceinline__ float gate_slope(float c, int act) {
+  if (act == DISCO_ACT_SIGMOID) return fabsf(c) * (1.0f - fabsf(c));
+  if (act == DISCO_ACT_TANH) return 1.0f - c * c;
   return 1.0f;
 }
 
@@ -346,6 +358,10 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E, MODE), residual_bac
   __shared__ float4 lds[LANES > 64 ? 2 * (LANES / 64) : 1];
   // the vectors; after the last row, for rows of a wave or less, the column sums of the workgroup's row groups
   __shared__ float4 store[(W <= 8192 ? (ROWS > 3 ? ROWS : 3) * W : 4) / 4];
+  // The code of a row's gate in a scalar register, decoded where it is used: the join has no vector register to spare (float32 rows
+  // of 602: 262 us with code and value in vector registers, 252 so and before).  1024 lanes spill either way, and less without.
+  constexpr bool SCALAR = MODE == kJoin && LANES >= 64 && LANES < 1024;
+  const int one = a.act == DISCO_ACT_SIGMOID ? 0x3f800000 : 0;
   constexpr bool IN_LDS = W <= 8192, AHEAD = LANES == 512 && MODE == kJoin && (E == 12 || sizeof(TX) == 2);
   typedef RowPart<TX, LANES, E, ODD> PX;
   typedef RowPart<TY, LANES, E, ODD> PY;
@@ -438,14 +454,15 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E, MODE), residual_bac
       if constexpr (FULL) {
         PY::expand(cg, act, lane, a.width);
 #pragma unroll
-        for (int e = 0; e < E; ++e) act[e] = activate(act[e], a.act);
+        for (int e = 0; e < E; ++e) act[e] = gate_code(act[e], a.act);
       } else {
-        if (a.gate == DISCO_GATE_ROW) gate = activate(gate, a.act);
-        act[0] = gate;
+        if (a.gate == DISCO_GATE_ROW) gate = gate_code(gate, a.act);
+        if constexpr (SCALAR) gate = __int_as_float(__builtin_amdgcn_readfirstlane(__float_as_int(gate)));
+        act[0] = SCALAR ? gate_value(gate, one) : a.act == DISCO_ACT_SIGMOID && signbit(gate) ? 1.0f + gate : gate;
       }
     }
     if (FULL) { fetch_sum(row); cx = rx; cdo = rdo; cdh = rdh; mean2 = m2; rstd2 = r2; }
-    const auto gated = [&](int e) { return act[FULL ? e : 0]; };
+    const auto gated = [&](int e) { return FULL ? gate_value(act[FULL ? e : 0], one) : act[0]; };
     if (BLOCK && a.dout) {
       PX::expand(cdo, d, lane, a.width);
     } else {
@@ -483,13 +500,17 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E, MODE), residual_bac
     if constexpr (BLOCK) {
       float s[3] = {0.0f, 0.0f, 0.0f};
       float dg[FULL ? E : 1], A[E], B[E];
+      if constexpr (SCALAR) {
+        asm volatile("" : "+s"(gate));
+        act[0] = gate_value(gate, one);
+      }
       vector(0, A);
       vector(1, B);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float t = d[e] * fmaf(u1[e], A[e], B[e]);
         s[2] += t;
-        if constexpr (FULL) dg[e] = t * activate_slope(act[e], a.act);
+        if constexpr (FULL) dg[e] = t * gate_slope(act[e], a.act);
         d[e] *= gated(e);
         P1[e] = fmaf(d[e], u1[e], P1[e]);
         P2[e] += d[e];
@@ -501,7 +522,7 @@ __global__ __launch_bounds__(residual_back_threads(LANES, E, MODE), residual_bac
         if (a.dg) PY::store(dg, static_cast<TY*>(a.dg) + row * a.lddg, lane, a.width);
       if (a.post || (!FULL && a.dg)) row_sum<LANES, 3>(s, lds, turn);
       if (!FULL && a.dg && lane == 0)
-        static_cast<TY*>(a.dg)[row * a.lddg] = (TY)(s[2] * activate_slope(gate, a.act));
+        static_cast<TY*>(a.dg)[row * a.lddg] = (TY)(s[2] * gate_slope(gate, a.act));
       if (a.dy) {
         if (a.post) {
           const float mp = a.post == DISCO_NORM_LAYER ? s[1] * a.inv_width : 0.0f, mpu = s[0] * a.inv_width;

@@ -77,9 +77,19 @@ __global__ __launch_bounds__(1024) void k_residual_finish(const FinishArgs a) {
   if (slice != 0 || c >= a.width) return;
   double gate = 1.0, slope = 0.0;
   if (a.channel) {
-    if (a.act == DISCO_ACT_SIGMOID) { gate = 1.0 / (1.0 + exp(-g)); slope = gate * (1.0 - gate); }
-    else if (a.act == DISCO_ACT_TANH) { gate = tanh(g); slope = 1.0 - gate * gate; }
-    else { gate = g; slope = 1.0; }
+    // slopes from the exponential: 1 - gate would cancel
+    if (a.act == DISCO_ACT_SIGMOID) {
+      const double e = exp(-fabs(g)), r = 1.0 / (1.0 + e);
+      gate = g < 0.0 ? e * r : r;
+      slope = e * r * r;
+    } else if (a.act == DISCO_ACT_TANH) {
+      const double e = exp(-2.0 * fabs(g)), r = 1.0 / (1.0 + e);
+      gate = tanh(g);
+      slope = 4.0 * e * r * r;
+    } else {
+      gate = g;
+      slope = 1.0;
+    }
   }
   if (a.dw1) param_put(a.dw1, a.param_type, c, scale * gate * P1);
   if (a.db1) param_put(a.db1, a.param_type, c, scale * gate * P2);

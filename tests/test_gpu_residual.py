@@ -707,3 +707,24 @@ def test_the_blocks_output_may_change_where_no_gradient_reads_it(stream, block, 
         b.detach().add_(1.0)
         with pytest.raises(RuntimeError, match="modified"):
             sum(o.sum() for o in (out if isinstance(out, tuple) else (out,))).backward()
+
+
+@pytest.mark.parametrize("stream,block", [("f32", "f32"), ("f32", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("gate", ["full", "row", "channel"])
+@pytest.mark.parametrize("F", [13, 64, 700, 1200, 2100, 9000])
+def test_the_slope_of_open_and_closed_gates(stream, block, gate, F, monkeypatch):
+    """The slope a (1 - a) of a sigmoid keeps its relative accuracy where 1 - a is small: e = exp(-|g|) is off by 2 u, 1 + e by u,
+    its reciprocal by 2 u and their product by u; the smaller of a and 1 - a then by 6 u, the larger by 7 u and their product by
+    14 u.  The 256 u of a gradient's terms hold that, here with the slope among their factors.  (Float64's own a (1 - a) would
+    cancel as well.)"""
+    def exact(g, act):
+        e = torch.exp(-g.abs())
+        return torch.sigmoid(g), e / (1 + e) ** 2
+
+    monkeypatch.setitem(globals(), "act64", exact)
+    s = make(24, F, stream, block, gate=gate, seed=95)
+    g = torch.tensor([0.0, 0.5, 4.0, 8.0, 10.0, 12.0, 14.0, 16.0, 18.0, 24.0, 40.0, 60.0], device=DEV)
+    g, t = torch.cat([g, -g]), s["t"]["gate"]
+    t.copy_(g.repeat(F)[:F] if gate == "channel" else g[:, None].expand(24, t.shape[1]))
+    v, m = formula(s)["gate"]
+    near(train(s)[2]["gate"], (v, m * exact(t.double(), None)[1]), "d_gate")
