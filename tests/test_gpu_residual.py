@@ -728,3 +728,30 @@ def test_the_slope_of_open_and_closed_gates(stream, block, gate, F, monkeypatch)
     t.copy_(g.repeat(F)[:F] if gate == "channel" else g[:, None].expand(24, t.shape[1]))
     v, m = formula(s)["gate"]
     near(train(s)[2]["gate"], (v, m * exact(t.double(), None)[1]), "d_gate")
+
+
+# rows, width: more than twice as many rows as a launch has workgroups for rows of two waves and more (by width 1536, 1024, 512,
+# 512, 256, 256 and 256 in the backward), and no multiple of that
+TURNS = [(3301, 1100), (2301, 1999), (1301, 2500), (1301, 4096), (701, 5001), (701, 8192), (701, 8193)]
+
+
+@pytest.mark.parametrize("n,F", TURNS)
+@pytest.mark.parametrize("stream,block", [("f32", "f32"), ("bf16", "bf16"), ("f32", "f16")])
+@pytest.mark.parametrize("gate", [None, "row", "full"])
+def test_workgroups_that_take_several_rows(n, F, stream, block, gate):
+    """One row after the other in a workgroup of several waves: column sums that go on, the two buffers of the row sums in turn,
+    the next row's loads under way (half rows and rows of 4097 to 6144 without a gate for each element)."""
+    check(make(n, F, stream, block, "f32", "layer", "rms", gate, gate and "sigmoid", seed=101))
+
+
+@pytest.mark.parametrize("n,F", TURNS)
+@pytest.mark.parametrize("stream,block", [("f32", "f32"), ("f16", "f16"), ("f32", "bf16")])
+def test_workgroups_that_norm_several_rows(n, F, stream, block):
+    s = make(n, F, stream, block, post=None, pre="layer", gate=None, scale="number", seed=102)
+    s["t"]["y"] = torch.zeros_like(s["t"]["y"])
+    want = formula(s, ("h",))
+    x, w, b = (s["t"][k].clone().requires_grad_() for k in ("x", "pre_weight", "pre_bias"))
+    h = ops.row_norm(x, w, b, kind="layer", eps=EPS, dtype=T[block])
+    near(h, want["h"], "h")
+    for k, g in zip(("x", "pre_weight", "pre_bias"), torch.autograd.grad(h, (x, w, b), s["dh"])):
+        near(g, want[k], "d_" + k)
