@@ -337,3 +337,21 @@ def test_two_gradients_into_one_view_with_gaps_are_refused():
     want = norm64(pair, 2)
     check_norm(ops.clip_grads(pair, 0.5, out=[pair[0], wide[:, 50:98]]), want)
     check_clip([keep, grads[1]], [wide[:, :48], wide[:, 50:98]], 0.5, want)
+
+
+@pytest.mark.parametrize("p", [2.0, 1.0, math.inf])
+@pytest.mark.parametrize("top,most", [(0.05, 0.3), (3e38, 1e-3), (1e-30, 1e-33), (1e30, 1e-4)])
+def test_the_factor_is_not_rounded(p, top, most):
+    """Factor and product are float64 (the factor beside gradients near float32's end is no normal float32): a clipped value is
+    rounded once, to float32, and once more to a narrower output: U, and half a step of that."""
+    base = torch.rand(5000, generator=torch.Generator(device=DEV).manual_seed(41), device=DEV) * top
+    grads = [base, base[:77].bfloat16()]
+    norm = norm64(grads, p)
+    factor = min(1.0, most / (norm + 1e-6))
+    for dtypes in ((torch.float32, torch.float32), (torch.float32, torch.bfloat16)):
+        to = [torch.empty_like(g, dtype=t) for g, t in zip(grads, dtypes)]
+        ops.clip_grads(grads, most, p, out=to)
+        for g, o in zip(grads, to):
+            want = g.double() * factor
+            half = U + (torch.finfo(o.dtype).eps / 2 if o.dtype != torch.float32 else 0.0)
+            assert ((o.double() - want).abs() <= half * want.abs() * (1 + 1e-6) + torch.finfo(o.dtype).smallest_normal * torch.finfo(o.dtype).eps).all()
