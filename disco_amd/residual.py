@@ -5,7 +5,8 @@
 
 and the norm before the first block (``row_norm``).  Both are differentiable in every tensor.  The reference normalises
 hidden layers with stock BatchNorm (/root/reference/models/basicgnn_large.py:119-133) and has no residual blocks; deep
-networks need them.  The arguments are checked here; the autograd node is disco_torch.cpp's.  There is no CPU fallback.
+networks need them.  The arguments are checked here; the autograd node is disco_torch.cpp's.  Sums of squares are float32: entries
+up to about 1e17.  Second and forward-mode derivatives are refused.  There is no CPU fallback.
 """
 from __future__ import annotations
 

@@ -368,7 +368,8 @@ int disco_anchor_max_f32(const float* T, int64_t n, int64_t ldt, int64_t width, 
  * have unit stride and rows need no alignment beyond their element's.  gate: [rows, width] (FULL, block type), [rows]
  * at ld_gate (ROW, block type) or [width] (CHANNEL, parameter type).  Types: stream_type of x, out and their gradients,
  * block_type of y, h, gate and theirs -- equal, or float32 with a 16-bit block -- and param_type of every vector.
- * Statistics and sums are float32 or float64; values are rounded to their type once.  A NaN or infinity stays in its row
+ * Statistics and sums are float32 or float64; values are rounded to their type once.  A row's sum of squares has to stay
+ * inside float32 (entries below about 1e17): beyond it a row normalises to zeros.  A NaN or infinity stays in its row
  * (and in the parameter gradients).  No counterpart in the reference, which normalises hidden layers with stock BatchNorm
  * (/root/reference/models/basicgnn_large.py:119-133) and has no residual blocks. */
 enum disco_dtype { DISCO_F32 = 0, DISCO_F16 = 1, DISCO_BF16 = 2 };
