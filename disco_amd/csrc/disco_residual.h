@@ -69,15 +69,14 @@ inline int residual_mode(bool block, int gate) { return !block ? kNormOnly : gat
 // ... of the backward: waves of a SIMD, which share its 512 registers.  An element of a lane needs 10 to 15 of them in the join and
 // 12 to 16 with a gate of its own, beside some 25 that every variant needs: four waves at 4 elements, four at 8 (three gated),
 // three at 12 (two gated, two where a row's sums pass through LDS of four waves and more), two at 16.  The norm alone needs 7 an
-// element and has room for four; from 12 on it is faster with fewer, whose rows meet less in memory, but for the eight waves of
-// 512 lanes.  One call's gradients over 60 M elements, us, with the number taken | with its neighbour:
+// element and has room for four; from 12 on it measured faster with fewer, but for rows of eight waves (512 lanes).  One call's gradients over 60 M elements, us, with the number taken | with its neighbour:
 //   norm   float32 rows of 602 (12 elements) 151 with 3 | 162 with 4, of 1000 (16) 155 with 2 | 161 with 3;
 //          half rows of 1433 (128 lanes, 12) 99 with 2 | 110 with 3, of 5000 (512 lanes, 12) 88 with 4 | 130 with 2
 //   join   float32 rows of 2500 (256 lanes, 12) 295 with 2 | 385 with 3, of 602 307 with 3 | 301 with 2; half rows of 602 169 with 3 |
 //          182 with 2, of 4096 (16) 165 with 2 | 223 with 1; a float32 stream with bfloat16 blocks of 1200 281 with 3 | 230 with 2
 //   gated  float32 rows of 602 392 with 2 | 459 with 3, of 1800 (256 lanes, 8) 408 with 3 | 412 with 4, of 4096 379 with 2 | 440 with 1
 // Where a neighbour is ahead here it spills less: 12 elements in three waves put 1 to 24 registers into scratch in most types,
-// rows of 8 to 32 half values (8 elements, four waves) 13 to 32, 1024 lanes up to 311; no other variant more than 10.
+// rows of up to 32 half values (8 elements, three or four waves) 13 to 32, 1024 lanes up to 311; no other variant more than 10.
 constexpr int residual_back_waves(int lanes, int elems, int mode) {
   return lanes == 1024 || elems <= 4 ? 4
          : mode == kNormOnly ? (elems <= 8 ? 4 : elems > 12 || lanes == 128 ? 2 : lanes == 512 ? 4 : 3)
