@@ -335,8 +335,8 @@ bool known(const Tensor& t) {
 // the kernels may walk the pair as it lies.
 bool walkable(const Tensor& g, const Tensor& o) {
   if (g.is_neg() || o.is_neg()) return false;      // negated when read: an operator that writes cannot take them
-  if (g.numel() == 0) return true;
-  return g.is_non_overlapping_and_dense() && (o.is_same(g) || o.strides() == g.strides() || (o.is_contiguous() && g.is_contiguous()));
+  if (g.sym_numel() == 0) return true;
+  return g.is_non_overlapping_and_dense() && (o.is_same(g) || o.sym_strides() == g.sym_strides() || (o.is_contiguous() && g.is_contiguous()));
 }
 
 // The norm over the gradients; with `out` also their clipping into it (out may be the list itself).  No value where the
@@ -352,11 +352,11 @@ std::optional<Tensor> gradient_norm(const std::vector<Tensor>& grads, const std:
   const auto device = grads[0].device();
   for (size_t i = 0; i < n; ++i) {
     const Tensor& g = grads[i];
-    if (g.layout() != at::kStrided || g.device() != device || !known(g) || (g.numel() > 0 && !g.is_non_overlapping_and_dense())) return std::nullopt;
+    if (g.layout() != at::kStrided || g.device() != device || !known(g) || (g.sym_numel() > 0 && !g.is_non_overlapping_and_dense())) return std::nullopt;
     if (!out) continue;
     const Tensor& o = (*out)[i];
     if (!o.is_same(g) && (o.layout() != at::kStrided || o.device() != device || (o.scalar_type() != g.scalar_type() && o.scalar_type() != at::kFloat) ||
-                          o.sizes() != g.sizes()))
+                          o.sym_sizes() != g.sym_sizes()))
       return std::nullopt;
     if (!walkable(g, o)) return std::nullopt;
   }

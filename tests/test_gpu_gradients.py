@@ -355,3 +355,17 @@ def test_the_factor_is_not_rounded(p, top, most):
             want = g.double() * factor
             half = U + (torch.finfo(o.dtype).eps / 2 if o.dtype != torch.float32 else 0.0)
             assert ((o.double() - want).abs() <= half * want.abs() * (1 + 1e-6) + torch.finfo(o.dtype).smallest_normal * torch.finfo(o.dtype).eps).all()
+
+
+@pytest.mark.parametrize("dynamic", [False, True])
+def test_compiled_clipping(dynamic):
+    f = torch.compile(lambda g, o: (ops.clip_grads(g, 0.5, out=o), ops.grad_norm(o)), backend="aot_eager", dynamic=dynamic)
+    try:
+        for n in (100, 77, 3000):
+            grads = make([(n, 3), n], DTYPES[:2], seed=n)
+            got, want = ([torch.empty_like(g, dtype=torch.float32) for g in grads] for _ in range(2))
+            a, b = f(grads, got)
+            assert torch.equal(a, ops.clip_grads(grads, 0.5, out=want)) and torch.equal(b, ops.grad_norm(want))
+            assert all(torch.equal(x, y) for x, y in zip(got, want))
+    finally:
+        torch._dynamo.reset()
