@@ -14,6 +14,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/util/SmallVector.h>
+#include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
@@ -490,6 +491,13 @@ TORCH_LIBRARY_IMPL(disco_amd, CUDA, m) {
   m.impl("residual_norm_backward", &backward_op);
   m.impl("grad_norm", &norm_op);
   m.impl("grad_clip", &clip_op);
+}
+
+// Called by themselves (a recorded graph that is differentiated again) they have no derivative, and say so.
+TORCH_LIBRARY_IMPL(disco_amd, Autograd, m) {
+  m.impl("residual_norm_forward", torch::autograd::autogradNotImplementedFallback());
+  m.impl("residual_norm_backward", torch::autograd::autogradNotImplementedFallback());
+  m.impl("grad_norm", torch::autograd::autogradNotImplementedFallback());
 }
 
 TORCH_LIBRARY_IMPL(disco_amd, Meta, m) {

@@ -755,3 +755,15 @@ def test_workgroups_that_norm_several_rows(n, F, stream, block):
     near(h, want["h"], "h")
     for k, g in zip(("x", "pre_weight", "pre_bias"), torch.autograd.grad(h, (x, w, b), s["dh"])):
         near(g, want[k], "d_" + k)
+
+
+def test_a_recorded_graph_is_not_differentiated_again():
+    """The operators that a trace holds have no derivative of their own: differentiating their results raises."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w = torch.randn(9, 12, device=DEV), torch.randn(12, device=DEV, requires_grad=True)
+    with torch.no_grad():
+        graph = make_fx(lambda a, b: (ops.residual_norm(a, a, post="rms", post_weight=b), ops.grad_norm([a, b])))(x, w)
+    for got, want in zip(graph(x, w), (ops.residual_norm(x, x, post="rms", post_weight=w), ops.grad_norm([x, w]))):
+        assert torch.equal(got, want)
+        with pytest.raises(RuntimeError, match="not implemented"):
+            got.sum().backward()
